@@ -258,6 +258,105 @@ int vxc_accept(const float *P, long long p_seq, long long p_pos, const float *Q,
                const int *seq_id, const int *pos0, int *n_acc, int *next, void *workspace,
                size_t workspace_bytes, void *stream);
 
+/* ---- paged 8-bit KV cache ------------------------------------------------------
+ * Keys and values of one layer in blocks of `block_size` tokens, one byte per
+ * element, with one fp32 scale for each (block, kv head) of K and one of V:
+ * element = code * scale.  A request's tokens lie in the blocks its row of a
+ * block table names, token p in entry p / block_size at offset
+ * p % block_size; `slot` = block * block_size + offset names one token of the
+ * cache.  The reference keeps one fp32 cache [layer][n_ctx][kv_dim] per model
+ * (src/model.c:404-411) and has no counterpart.
+ *
+ * All arrays are device memory of the calling thread's current device (k and v
+ * 16-byte aligned, the others by their element type); nothing is copied to the
+ * host and nothing is allocated, so every call can be captured in a CUDA
+ * graph.  Calls are ordered by their streams only: a call that writes a cache
+ * or a table may not overlap another call on the same one.
+ * Out-of-range device data (a slot, a table entry, a length) never leads to an
+ * access outside the arrays; it raises the device error word, as stated at
+ * each call. */
+#define VXC_KV8_INT8 1    /* signed 8-bit integers, codes -127..127 */
+#define VXC_KV8_E4M3 2    /* 8-bit floats, 4 exponent and 3 significand bits, |code| <= 448 */
+typedef struct {
+    int type;                       /* VXC_KV8_INT8 or VXC_KV8_E4M3 */
+    int n_blocks, block_size;       /* block_size a multiple of 16, 16..256 */
+    int n_kv_heads, head_dim;       /* head_dim 32, 64, 96 or 128 */
+    void *k, *v;                    /* [n_blocks][n_kv_heads][block_size][head_dim] bytes */
+    float *k_scale, *v_scale;       /* [n_blocks][n_kv_heads], zero at first */
+} vxc_kv8;
+
+/* Block tables and slot maps from request lengths.  Request r (r < n_req <=
+ * VXC_KV8_MAX_REQ) has d_len[r] cached tokens and gets d_new[r] more; it then
+ * needs ceil((len + new) / block_size) blocks.  It holds the d_held[r] blocks
+ * in d_table[r][0..held) ([n_req][max_blocks] ints).  Missing blocks are taken
+ * from the front of the queue of free blocks, in request order; surplus ones
+ * (a shorter length: tokens dropped, or a request that ended, len = new = 0)
+ * go to its back, in request and table order, and their entries become -1.
+ * The queue is the ring d_free[n_blocks] with d_state = {front, count,
+ * status}; a block put back by a call can be taken by the next one.  d_table,
+ * d_held, d_free and d_state are updated in place.
+ * Outputs: d_row0[n_req + 1], the first row of each request's new tokens and
+ * their total, and d_slot[n_rows], the slot of every new token, request after
+ * request; entries behind the last token are -1.
+ * d_state[2] becomes 0, or the call changes neither the tables nor the queue,
+ * sets d_row0 to 0 and d_slot to -1, and d_state[2] to 1: fewer free blocks
+ * than needed; 2: a request longer than max_blocks blocks; 3: a negative
+ * length, more than n_rows new tokens, or held blocks and a queue that do not
+ * fit n_blocks (2 and 3 also raise the device error word).
+ * One launch. */
+#define VXC_KV8_MAX_REQ 8192
+int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks, int max_blocks,
+                   int *d_table, int *d_held, int *d_free, int *d_state, int n_rows, int *d_row0, int *d_slot,
+                   void *stream);
+
+/* Quantise n_rows K and V rows (fp32, row i at k + i * ldk and v + i * ldv, the
+ * heads side by side, kv heads x head_dim floats; 16-byte aligned, ld a
+ * multiple of 4) into the tokens d_slot[i] (-1: the row is skipped).  For each
+ * block with a row and each head, for K and V alike:
+ *   s = max(scale, the smallest power of two with |x| <= max code * s for the
+ *       new rows), scale counting as 0 when the call writes the block's first
+ *       token: the block then starts anew;
+ *   if s grew from a scale > 0, the block's other codes are rounded again to
+ *       code * old / s;
+ *   the rows' codes are x / s to nearest, ties to even, and the scale is s.
+ * (Powers of two: dividing by s is exact, a growing scale shifts the codes, so
+ * an element is off by at most one step of s however often s grew.)
+ * The rows of one block stand together in d_slot, with no other or skipped
+ * row between them, as vxc_kv8_tables writes them; of two rows with the same slot
+ * the later one is kept.  A slot outside the cache is skipped and raises the
+ * device error word, a NaN or infinite element is stored as 0 and raises it.
+ * n_rows <= VXC_KV8_MAX_ROWS; 0 rows is no launch. */
+#define VXC_KV8_MAX_ROWS (1 << 22)
+int vxc_kv8_append(const vxc_kv8 *kv, const float *k, long long ldk, const float *v, long long ldv,
+                   const int *d_slot, int n_rows, void *stream);
+
+/* Scratch bytes vxc_kv8_attn needs for these sizes (0 for sizes it refuses).
+ * Nothing in it has to be initialised; calls that may overlap on the GPU need
+ * scratch of their own. */
+size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new,
+                                    int max_blocks);
+
+/* Causal attention of the new rows over the cache (their own tokens included:
+ * append them first).  Request r's rows are d_row0[r]..d_row0[r + 1] - 1, at
+ * most max_new of them, at positions d_pos[r], d_pos[r] + 1, ...; row i of
+ * head h is
+ *   out[i * ldo + h * hd ..] = sum_j softmax_j(scale * q_i,h . k_j) v_j
+ * over the request's tokens j <= position, kv head h / (n_heads / kv heads)
+ * (reference src/model.c:299-338 over its fp32 cache).  fp32 in and out,
+ * q rows of ldq and out rows of ldo floats (16-byte aligned, ld a multiple of
+ * 4); out may not overlap q.  Products are exact to fp32 level: codes are
+ * exact in fp16, queries and weights are split into two fp16 parts, sums and
+ * softmax are fp32.
+ * A row whose position is negative sees no token and is set to 0.  Rows behind
+ * d_row0[n_req] are left as they were.  Bytes of the cache behind a request's
+ * last token are not used, whatever they hold.  These raise the device error
+ * word: more than max_new or n_rows rows, or tokens behind max_blocks blocks
+ * (the rows in question are left as they were), and a table entry outside the
+ * cache (its tokens count as masked). */
+int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, int n_heads, float scale, const int *d_table,
+                 int max_blocks, const int *d_row0, const int *d_pos, int n_req, int n_rows, int max_new,
+                 float *out, long long ldo, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- device speculative-decoding engine --------------------------------------- */
 
 typedef struct vxc_spec vxc_spec;

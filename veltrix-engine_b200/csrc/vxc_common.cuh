@@ -28,6 +28,8 @@ void vxc_set_error(const char *fmt, ...);
 #define VXC_DERR_BAD_SHAPE 8u
 #define VXC_DERR_CTX_FULL 16u
 #define VXC_DERR_TIMEOUT_EPI 32u
+#define VXC_DERR_BAD_BLOCK 64u     // block table entry, slot or request length outside the paged cache
+#define VXC_DERR_NONFINITE 128u    // NaN or infinity appended to the paged cache
 
 __device__ __forceinline__ void vxc_flag_error(unsigned int *err, unsigned int code) {
     if (err) atomicOr(err, code);

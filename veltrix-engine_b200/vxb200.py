@@ -71,6 +71,14 @@ PROTOTYPES = {
     "vxc_accept": (ctypes.c_int, [_vp, ctypes.c_longlong, ctypes.c_longlong, _vp, ctypes.c_longlong,
                                   ctypes.c_longlong, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                   ctypes.c_uint64, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "vxc_kv8_tables": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp,
+                                      _vp, ctypes.c_int, _vp, _vp, _vp]),
+    "vxc_kv8_append": (ctypes.c_int, [_vp, _vp, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp, ctypes.c_int, _vp]),
+    "vxc_kv8_attn_workspace_bytes": (ctypes.c_size_t, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                       ctypes.c_int]),
+    "vxc_kv8_attn": (ctypes.c_int, [_vp, _vp, ctypes.c_longlong, ctypes.c_int, ctypes.c_float, _vp, ctypes.c_int, _vp,
+                                    _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_longlong, _vp,
+                                    ctypes.c_size_t, _vp]),
     "vxc_spec_create": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
     "vxc_spec_destroy": (None, [_vp]),
     "vxc_spec_probe": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, _vp]),
@@ -327,3 +335,39 @@ class QMat:
             self.close()
         except Exception:
             pass
+
+
+KV8_INT8, KV8_E4M3 = 1, 2
+
+
+class _KV8(ctypes.Structure):
+    """vxc_kv8 (include/veltrix_cuda.h)."""
+    _fields_ = [("type", ctypes.c_int), ("n_blocks", ctypes.c_int), ("block_size", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("k", _vp), ("v", _vp), ("k_scale", _vp),
+                ("v_scale", _vp)]
+
+
+def kv8_tables(len_ptr, new_ptr, n_req, block_size, n_blocks, max_blocks, table_ptr, held_ptr, free_ptr, state_ptr,
+               n_rows, row0_ptr, slot_ptr, stream=0):
+    """vxc_kv8_tables: block tables and slot maps from request lengths, on the device."""
+    check(lib().vxc_kv8_tables(len_ptr, new_ptr, n_req, block_size, n_blocks, max_blocks, table_ptr, held_ptr,
+                               free_ptr, state_ptr, n_rows, row0_ptr, slot_ptr, stream), "vxc_kv8_tables")
+
+
+class KV8:
+    """One layer's paged 8-bit K/V cache (vxc_kv8) over device buffers that the caller owns."""
+
+    def __init__(self, ctype, n_blocks, block_size, n_kv_heads, head_dim, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr):
+        self.c = _KV8(ctype, n_blocks, block_size, n_kv_heads, head_dim, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr)
+        self.ref = ctypes.byref(self.c)
+
+    def append(self, k_ptr, ldk, v_ptr, ldv, slot_ptr, n_rows, stream=0):
+        check(lib().vxc_kv8_append(self.ref, k_ptr, ldk, v_ptr, ldv, slot_ptr, n_rows, stream), "vxc_kv8_append")
+
+    def attn_workspace_bytes(self, n_heads, n_req, n_rows, max_new, max_blocks):
+        return lib().vxc_kv8_attn_workspace_bytes(self.ref, n_heads, n_req, n_rows, max_new, max_blocks)
+
+    def attn(self, q_ptr, ldq, n_heads, scale, table_ptr, max_blocks, row0_ptr, pos_ptr, n_req, n_rows, max_new,
+             out_ptr, ldo, ws_ptr, ws_bytes, stream=0):
+        check(lib().vxc_kv8_attn(self.ref, q_ptr, ldq, n_heads, scale, table_ptr, max_blocks, row0_ptr, pos_ptr, n_req,
+                                 n_rows, max_new, out_ptr, ldo, ws_ptr, ws_bytes, stream), "vxc_kv8_attn")
