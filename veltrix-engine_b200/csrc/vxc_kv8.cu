@@ -4,6 +4,7 @@
 // src/model.c:404-411.)
 #include "vxc_kv8.cuh"
 
+#include <atomic>
 #include <climits>
 #include <cooperative_groups.h>
 
@@ -37,6 +38,39 @@ int vxc_kv8_check(const vxc_kv8 *kv, const char *who) {
         return -4;
     }
     return 0;
+}
+
+// The limit is per kernel and device and only ever raised; a kernel that has
+// it on a device is remembered, since asking costs a launch's time.
+cudaError_t kv8_allow_smem(const void *kernel, size_t bytes) {
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    struct Entry {
+        std::atomic<const void *> kernel;
+        std::atomic<size_t> bytes[64];
+    };
+    static Entry seen[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    Entry *own = nullptr;
+    for (Entry &s : seen) {
+        const void *k = s.kernel.load(std::memory_order_acquire);
+        if (!k && s.kernel.compare_exchange_strong(k, kernel)) k = kernel;
+        if (k == kernel) {
+            own = &s;
+            break;
+        }
+    }
+    if (own && dev < 64 && own->bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e == cudaSuccess && (size_t)fa.maxDynamicSharedSizeBytes < bytes)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && own && dev < 64) {
+        size_t have = own->bytes[dev].load();
+        while (have < bytes && !own->bytes[dev].compare_exchange_weak(have, bytes)) {}
+    }
+    return e;
 }
 
 // ---------------------------------------------------------------------------
@@ -229,16 +263,15 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
         return -4;
     }
     if (block_size < 16 || block_size > KV8_MAX_BS || block_size % 16 || n_blocks < 1 || max_blocks < 1 ||
-        (long long)n_blocks * block_size > INT_MAX || (long long)max_blocks * block_size > INT_MAX) {
+        (long long)n_blocks * block_size > INT_MAX || (long long)max_blocks * block_size > KV8_MAX_TOKENS) {
         vxc_set_error("vxc_kv8_tables: %d blocks of %d tokens, %d per request", n_blocks, block_size, max_blocks);
         return -4;
     }
     if (int rc = vxc_require_device()) return rc;
     const size_t smem = (size_t)(4 * n_req + 3) * sizeof(int);
     const int nc = n_rows >= TB_CLUSTER_ROWS ? TB_CLUSTER : 1;
-    if (smem > 44 * 1024)   // the static arrays take the rest of the default 48 KB
-        VXC_CUDA_OK(cudaFuncSetAttribute(k_kv8_tables, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)((4 * VXC_KV8_MAX_REQ + 3) * sizeof(int))));
+    // the static arrays take the rest of the default 48 KB
+    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (4 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
     VXC_CUDA_OK(kv8_launch(k_kv8_tables, dim3(nc), dim3(TB_THREADS), smem, (cudaStream_t)stream, nc, d_len, d_new,
                            n_req, block_size, n_blocks, max_blocks, d_table, d_held, d_free, d_state, n_rows, d_row0,
                            d_slot, vxc_device_error_ptr()));

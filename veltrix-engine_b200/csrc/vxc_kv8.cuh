@@ -5,7 +5,8 @@
 #include "vxc_internal.h"
 #include "vxc_ptx.cuh"
 
-#define KV8_MAX_BS 256   // tokens per block at most
+#define KV8_MAX_BS 256               // tokens per block at most
+#define KV8_MAX_TOKENS (1ll << 30)   // tokens of a table row at most (positions and splits are ints)
 
 // Largest code of a type.
 __host__ __device__ constexpr float kv8_qmax(int type) { return type == VXC_KV8_INT8 ? 127.0f : 448.0f; }
@@ -75,5 +76,7 @@ static cudaError_t kv8_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t
     return e;
 }
 
+// Lets `kernel` be launched with `bytes` of dynamic shared memory on the current device.
+cudaError_t kv8_allow_smem(const void *kernel, size_t bytes);
 // 0, or -4 with the error set: the fields of a cache (host side).
 int vxc_kv8_check(const vxc_kv8 *kv, const char *who);

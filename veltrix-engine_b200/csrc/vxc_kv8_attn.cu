@@ -3,8 +3,6 @@
 //   out_i,h = sum_j softmax_j(scale q_i,h . k_j) v_j,  j <= position of row i
 #include "vxc_kv8.cuh"
 
-#include <climits>
-
 struct Kv8AttnArgs {
     vxc_kv8 kv;
     const float *q;
@@ -18,81 +16,482 @@ struct Kv8AttnArgs {
     int n_req, n_rows, max_new;
     float *out;
     long long ldo;
+    float *part;        // records of the splits
+    int S, sl_min;      // splits per request at most, tokens per split at least
     unsigned int *err;
 };
 
-// One warp per (row, head), lanes over 32 tokens for the scores and over the
-// head dim for the output; online softmax, all in fp32.
-template <int TYPE, int HD>
-__global__ void __launch_bounds__(128) k_kv8_attn_rows(const Kv8AttnArgs a) {
-    __shared__ __align__(16) float qs[4][HD];
+// ---------------------------------------------------------------------------
+// Few queries per kv head (decode and small verify steps): split over the
+// context, warp-level tensor instructions.
+//
+// CTA = (request, kv head, chunk of NQ queries) x one split of the request's
+// tokens.  Queries are the request's rows times the heads of the kv head,
+// query = row * G + head, so every byte of the split is read once for all.
+// Each of the 4 warps goes over every fourth tile of 16 tokens, with a softmax
+// state and an output of its own; the warps are joined at the end.
+//
+// Products.  mma m16n8k16 in fp16 with fp32 sums.  A code is exact in fp16.  A
+// query row is scaled by a power of two and split into two fp16 parts, hi and
+// lo (22 bits); so are the weights.
+//   NQ = 8: rows 0-7 of the instruction's 16 are hi, rows 8-15 are lo, and
+//     their two sums are added: one instruction does both products.
+//   NQ = 16: two instructions into the same sums, hi and lo.
+// Layouts.  The sum over the head dim may go in any order, so lane t of a quad
+// takes the pieces of a K row that it can load as whole words (kv8_k_at), and
+// the query's fragment is loaded in the same order.  Likewise the output's
+// columns: lane group g takes pieces of a V row (kv8_v_at).  So every byte goes
+// by cp.async to the ring slot of the lane that uses it, and back from there
+// without a bank conflict; no lane reads another's bytes and the ring needs no
+// barrier.  Scores come out where the weights' fragment wants them: lane (g, t)
+// has tokens 2t, 2t+1, 2t+8, 2t+9 of query g, and loads V of just these.
+// Softmax in base 2 with two running maxima per query: m of the scores s, for
+// the sum l of 2^(s - m), and mv of s + log2(v_scale), the reference of the
+// weights w = 2^(s - mv) v_scale 2^KV8_HEAD that multiply the codes of V: a
+// weight keeps its 22 bits whatever the scales of the other blocks are.  They
+// follow the true maximum only when it is over KV8_LAG ahead, so the output is
+// seldom rescaled.
+// Tokens behind the request's last one and blocks outside the cache are read
+// as zeros (cp.async's zero fill), so nothing of theirs reaches a product.
+// ---------------------------------------------------------------------------
+#define KV8_HEAD 10.0f   // weights up to 2^(10 + 5): in fp16's range with 2^-34 of the largest as last place
+#define KV8_LAG 5.0f
+#define FEW_STAGES 4     // 16-token tiles in flight per warp
+
+// Bytes that one cp.async brings, and the offset of piece c in a row.
+template <int HD>
+struct Kv8Piece {
+    static constexpr int K = HD % 64 == 0 ? 16 : 8, NK = HD / 4 / K;                    // of a K row, lane t of a quad
+    static constexpr int V = HD == 128 ? 16 : HD == 64 ? 8 : 4, NV = HD / 8 / V;        // of a V row, lane group g
+    static __device__ __forceinline__ int k_at(int c, int t) { return c * 4 * K + t * K; }
+    static __device__ __forceinline__ int v_at(int c, int g) { return c * 8 * V + g * V; }
+};
+
+template <int N>
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void *src, bool have) {
+    const int n = have ? N : 0;
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// a, b -> half2 of their fp16 roundings, and half2 of what is left
+__device__ __forceinline__ uint32_t split_h2(float a, float b, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Four codes -> two half2, bytes (0, 1) and (2, 3).  int8: the byte with its
+// sign bit flipped is the low byte of the half 1024 + 128 + code.
+template <int TYPE>
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &h01, uint32_t &h23) {
+    if (TYPE == VXC_KV8_INT8) {
+        const uint32_t x = w ^ 0x80808080u;
+        uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const __half2 ha = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+        h01 = *reinterpret_cast<const uint32_t *>(&ha);
+        h23 = *reinterpret_cast<const uint32_t *>(&hb);
+    } else {
+        h01 = kv8_e4m3x2_h2((uint16_t)(w & 0xFFFFu));
+        h23 = kv8_e4m3x2_h2((uint16_t)(w >> 16));
+    }
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A request's rows and tokens as the call's arguments and arrays allow them.
+struct Kv8Req {
+    int row0, T;     // first row; rows (clamped to n_rows, max_new and the table)
+    int pos;         // position of the first row
+    int kvlen;       // tokens the last row sees (0: none)
+    bool over;       // something was clamped
+};
+__device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
+    Kv8Req q;
+    const int r0 = a.row0[r], r1 = a.row0[r + 1];
+    q.pos = a.pos[r];
+    q.row0 = max(r0, 0);
+    long long T = (long long)r1 - r0;
+    const long long cap = (long long)a.max_blocks * a.kv.block_size;
+    const long long most = min(min((long long)a.max_new, (long long)a.n_rows - q.row0), cap - q.pos);
+    q.over = r0 < 0 || T > most;
+    T = r0 < 0 ? 0 : min(T, most);
+    q.T = (int)max(T, 0ll);
+    q.kvlen = q.T > 0 ? max(q.pos + q.T, 0) : 0;
+    return q;
+}
+
+// Splits of a request: enough for SL_min tokens each, at most S.
+__device__ __forceinline__ int kv8_splits(int kvlen, int sl_min, int S, int &SL) {
+    const int want = min(max((kvlen + sl_min - 1) / sl_min, 1), S);
+    SL = ((kvlen + want - 1) / want + 63) & ~63;
+    return SL > 0 ? (kvlen + SL - 1) / SL : 1;
+}
+
+// Records of the splits: [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum
+// of 2^(s - m) v.
+template <int TYPE, int HD, int NQ>
+__global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8AttnArgs a) {
+    using P = Kv8Piece<HD>;
+    constexpr int NR = NQ / 8;                 // query rows per lane
+    constexpr int KS = HD / 16;                // steps over the head dim
+    constexpr int NT = HD / 8;                 // column tiles of the output
+    constexpr int STAGE = HD * 32 + 16;        // a tile's codes, its two scales
+    extern __shared__ __align__(16) unsigned char sm[];
+    const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
     pdl_trigger();
     pdl_wait();
+    const int r = blockIdx.z, kvh = blockIdx.x % KH, q0 = (blockIdx.x / KH) * NQ, split = blockIdx.y;
+    const Kv8Req rq = kv8_req(a, r);
+    if (rq.over && blockIdx.x == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+    const int nq = rq.T * G;
+    if (q0 >= nq) return;
+    int SL;
+    const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
+    if (split >= ns) return;
+    // visible tokens of the chunk's last query end this CTA's range
+    const int p0 = split * SL, p1 = min(p0 + SL, rq.pos + (min(q0 + NQ, nq) - 1) / G + 1);
+
+    // queries: fragments hi (and lo), the factor of each row's scores
+    uint32_t qf[NR == 1 ? 1 : 2][KS][4];
+    float f[NR];
+    int lim[NR];   // last visible token
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int q = q0 + g + 8 * i;
+        const bool have = q < nq;
+        const int row = rq.row0 + (have ? q / G : 0), h = kvh * G + (have ? q % G : 0);
+        const float *x = a.q + (size_t)row * a.ldq + (size_t)h * HD;
+        float4 v[KS];
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int c = s / (P::K / 4), e = P::k_at(c, t) + 4 * (s % (P::K / 4));
+            v[s] = have ? *reinterpret_cast<const float4 *>(x + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[s].x), fabsf(v[s].y)), fmaxf(fabsf(v[s].z), fabsf(v[s].w))));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // the row's largest element into [2^13, 2^14)
+        const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
+        const float up = __uint_as_float((uint32_t)(267 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 13) << 23);
+        f[i] = a.scale * 1.4426950408889634f * down;
+        lim[i] = have ? rq.pos + q / G : -1;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            uint32_t l0, l1;
+            const uint32_t h0 = split_h2(v[s].x * up, v[s].y * up, l0), h1 = split_h2(v[s].z * up, v[s].w * up, l1);
+            if (NR == 1) {
+                qf[0][s][0] = h0, qf[0][s][1] = l0, qf[0][s][2] = h1, qf[0][s][3] = l1;
+            } else {
+                qf[0][s][i] = h0, qf[0][s][2 + i] = h1;
+                qf[NR - 1][s][i] = l0, qf[NR - 1][s][2 + i] = l1;
+            }
+        }
+    }
+
+    float o[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[NR], mv[NR], l[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) m[i] = mv[i] = -INFINITY, l[i] = 0.0f;
+
+    // tiles w, w + 4, ... of the range
+    const int ntile = p1 > p0 ? (p1 - p0 + 15) >> 4 : 0, nit = ntile > w ? (ntile - w + 3) >> 2 : 0;
+    unsigned char *ring = sm + w * (FEW_STAGES * STAGE);
+    const uint32_t ring_u = smem_u32(ring);
+    const int *trow = a.table + (size_t)r * a.max_blocks;
+    const int bs16 = bs >> 4;
+    int blk = (p0 / 16 + w) / bs16, off16 = (p0 / 16 + w) % bs16;   // of the next tile to issue
+    int p_issue = p0 + 16 * w;
+    int b_next = nit > 0 ? trow[blk] : -1;
+    uint32_t bad = 0;   // stages whose block is outside the cache
+    auto issue = [&](int it) {
+        if (it < nit) {
+            const int st = it % FEW_STAGES;
+            const bool ok = b_next >= 0 && b_next < a.kv.n_blocks;
+            bad = (bad & ~(1u << st)) | (ok ? 0u : 1u << st);
+            const size_t bh = (size_t)(ok ? b_next : 0) * KH + kvh;
+            const size_t at = (bh * bs + (size_t)off16 * 16) * HD;
+            const uint8_t *ks = (const uint8_t *)a.kv.k + at, *vs = (const uint8_t *)a.kv.v + at;
+            const uint32_t base = ring_u + st * STAGE;
+            const int live = ok ? rq.kvlen - p_issue : 0;   // tokens of the tile that exist
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < P::NK; c++)
+                    cp_async_zfill<P::K>(base + (n * P::NK + c) * 32 * P::K + lane * P::K,
+                                         ks + (n * 8 + g) * HD + P::k_at(c, t), n * 8 + g < live);
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const int tok = (n >> 1) * 8 + 2 * t + (n & 1);
+#pragma unroll
+                for (int c = 0; c < P::NV; c++)
+                    cp_async_zfill<P::V>(base + HD * 16 + (n * P::NV + c) * 32 * P::V + lane * P::V,
+                                         vs + tok * HD + P::v_at(c, g), tok < live);
+            }
+            if (lane < 2) cp_async_zfill<4>(base + HD * 32 + 4 * lane, (lane ? a.kv.v_scale : a.kv.k_scale) + bh, ok);
+            p_issue += 64;
+            off16 += 4;
+            while (off16 >= bs16) off16 -= bs16, blk++;
+            if (it + 1 < nit) b_next = trow[blk];
+        }
+        cp_commit();
+    };
+    if (nit > 0) {
+#pragma unroll 1
+        for (int i = 0; i < FEW_STAGES - 1; i++) issue(i);
+    }
+#pragma unroll 1
+    for (int it = 0; it < nit; it++) {
+        __syncwarp();   // the stage's scales have been read by every lane
+        const uint32_t was_bad = bad;
+        issue(it + FEW_STAGES - 1);
+        cp_wait<FEW_STAGES - 1>();
+        __syncwarp();
+        const unsigned char *stg = ring + (it % FEW_STAGES) * STAGE;
+        const float kscale = *reinterpret_cast<const float *>(stg + HD * 32);
+        const float vscale = *reinterpret_cast<const float *>(stg + HD * 32 + 4);
+        const bool is_bad = (was_bad >> (it % FEW_STAGES)) & 1u;
+        if (is_bad && lane == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+        // scores
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < P::NK; c++) {
+                uint32_t word[P::K / 4];
+                const unsigned char *src = stg + (n * P::NK + c) * 32 * P::K + lane * P::K;
+                if (P::K == 16) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                    word[0] = x.x, word[1] = x.y, word[P::K / 4 - 2] = x.z, word[P::K / 4 - 1] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    word[0] = x.x, word[1] = x.y;
+                }
+#pragma unroll
+                for (int e = 0; e < P::K / 4; e++) {
+                    const int s = c * (P::K / 4) + e;
+                    uint32_t b0, b1;
+                    codes_h2<TYPE>(word[e], b0, b1);
+                    mma16816(sc[n], qf[0][s], b0, b1);
+                    if (NR == 2) mma16816(sc[n], qf[NR - 1][s], b0, b1);
+                }
+            }
+        }
+        // weights: lane's tokens p, p + 1, p + 8, p + 9
+        const int p = p0 + 16 * (w + 4 * it) + 2 * t;
+        const float lv = lg2(vscale);
+        uint32_t wf[NR == 1 ? 1 : 2][4];
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const float fk = f[i] * kscale;
+            float s[4];
+            if (NR == 1) {
+                s[0] = sc[0][0] + sc[0][2], s[1] = sc[0][1] + sc[0][3];
+                s[2] = sc[1][0] + sc[1][2], s[3] = sc[1][1] + sc[1][3];
+            } else {
+                s[0] = sc[0][2 * i], s[1] = sc[0][2 * i + 1], s[2] = sc[1][2 * i], s[3] = sc[1][2 * i + 1];
+            }
+            const int end = is_bad ? -1 : lim[i];
+#pragma unroll
+            for (int k = 0; k < 4; k++) s[k] = p + (k & 1) + (k >> 1) * 8 <= end ? s[k] * fk : -INFINITY;
+            float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if (mx > m[i] + KV8_LAG || (m[i] == -INFINITY && mx > m[i])) {
+                l[i] *= ex2(m[i] - mx);   // 0 at first
+                m[i] = mx;
+            }
+            const float mxv = mx + lv;
+            float shrink = 1.0f;
+            if (mxv > mv[i] + KV8_LAG || (mv[i] == -INFINITY && mxv > mv[i])) {
+                shrink = ex2(mv[i] - mxv);
+                mv[i] = mxv;
+            }
+            if (__any_sync(0xffffffffu, shrink != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    if (NR == 1) {
+                        o[j][0] *= shrink, o[j][1] *= shrink, o[j][2] *= shrink, o[j][3] *= shrink;
+                    } else {
+                        o[j][2 * i] *= shrink, o[j][2 * i + 1] *= shrink;
+                    }
+                }
+            }
+            const float mref = m[i] == -INFINITY ? 0.0f : m[i];
+            const float c = vscale * ex2(fminf(mref - mv[i] + KV8_HEAD, 120.0f));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                s[k] = ex2(s[k] - mref);
+                l[i] += s[k];
+                s[k] *= c;
+            }
+            uint32_t l0, l1;
+            const uint32_t h0 = split_h2(s[0], s[1], l0), h1 = split_h2(s[2], s[3], l1);
+            if (NR == 1) {
+                wf[0][0] = h0, wf[0][1] = l0, wf[0][2] = h1, wf[0][3] = l1;
+            } else {
+                wf[0][i] = h0, wf[0][2 + i] = h1;
+                wf[NR - 1][i] = l0, wf[NR - 1][2 + i] = l1;
+            }
+        }
+        // weights times V: byte j of the lane's piece of tokens 2t, 2t+1, 2t+8, 2t+9 is column tile j
+        const unsigned char *vst = stg + HD * 16 + lane * P::V;
+#pragma unroll
+        for (int c = 0; c < P::NV; c++) {
+            uint32_t tok[4][P::V / 4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const unsigned char *src = vst + (n * P::NV + c) * 32 * P::V;
+                if (P::V == 16) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                    tok[n][0] = x.x, tok[n][P::V / 4 > 1 ? 1 : 0] = x.y;
+                    tok[n][P::V / 4 > 2 ? 2 : 0] = x.z, tok[n][P::V / 4 - 1] = x.w;
+                } else if (P::V == 8) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    tok[n][0] = x.x, tok[n][P::V / 4 - 1] = x.y;
+                } else {
+                    tok[n][0] = *reinterpret_cast<const uint32_t *>(src);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < P::V / 4; e++) {
+                uint32_t b0[4], b1[4];
+                codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x5140), b0[0], b0[1]);
+                codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x7362), b0[2], b0[3]);
+                codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x5140), b1[0], b1[1]);
+                codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int j = c * P::V + 4 * e + k;
+                    mma16816(o[j], wf[0], b0[k], b1[k]);
+                    if (NR == 2) mma16816(o[j], wf[NR - 1], b0[k], b1[k]);
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();   // the ring is free
+
+    // join the warps: unnormalised outputs in units of 2^m, maxima and sums
+    float *so = reinterpret_cast<float *>(sm);            // [4][NQ][HD + 4]
+    float *sml = so + 4 * NQ * (HD + 4);                  // [4][NQ][2]
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const float back = mv[i] == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv[i] - m[i] - KV8_HEAD, 126.0f), -126.0f));
+        float *dst = so + (w * NQ + g + 8 * i) * (HD + 4);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int c = j / P::V, e = j % P::V;
+            const float x = NR == 1 ? o[j][0] + o[j][2] : o[j][2 * i], y = NR == 1 ? o[j][1] + o[j][3] : o[j][2 * i + 1];
+            dst[P::v_at(c, 2 * t) + e] = x * back;
+            dst[P::v_at(c, 2 * t + 1) + e] = y * back;
+        }
+        if (t == 0) {
+            sml[(w * NQ + g + 8 * i) * 2] = m[i];
+            sml[(w * NQ + g + 8 * i) * 2 + 1] = l[i];
+        }
+    }
+    __syncthreads();
+    // one warp per query
+    for (int q = w; q < NQ && q0 + q < nq; q += 4) {
+        float M = -INFINITY, mw[4], L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) M = fmaxf(M, mw[k] = sml[(k * NQ + q) * 2]);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            mw[k] = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
+            L += mw[k] * sml[(k * NQ + q) * 2 + 1];
+        }
+        const int row = rq.row0 + (q0 + q) / G, h = kvh * G + (q0 + q) % G;
+        float *rec = a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
+        float *out = a.out + (size_t)row * a.ldo + (size_t)h * HD;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
+#pragma unroll
+        for (int d = lane; d < HD; d += 32) {
+            float x = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (mw[k] != 0.0f) x = fmaf(mw[k], so[(k * NQ + q) * (HD + 4) + d], x);
+            if (ns == 1) out[d] = x * inv;
+            else rec[4 + d] = x;
+        }
+        if (ns > 1 && lane == 0) *reinterpret_cast<float2 *>(rec) = make_float2(M, L);
+    }
+}
+
+// Joins the splits of the requests that have several: one warp per (row, head).
+template <int HD>
+__global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    pdl_wait();
     const int i = blockIdx.x, h = blockIdx.y * 4 + w;
-    if (i == 0 && h == 0 && lane == 0 && a.row0[a.n_req] > a.n_rows) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
-    if (h >= a.H || i >= a.row0[a.n_req] || i >= a.n_rows) return;
+    if (h >= a.H || i >= a.row0[a.n_req]) return;
     int lo = 0, hi = a.n_req;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (a.row0[mid] <= i) lo = mid; else hi = mid;
     }
-    const int r = lo, t = i - a.row0[r], bs = a.kv.block_size, KH = a.kv.n_kv_heads, kvh = h / (a.H / KH);
-    const long long last = (long long)a.pos[r] + t;   // last visible token
-    if (t < 0 || t >= a.max_new || last >= (long long)a.max_blocks * bs) {
-        if (lane == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
-        return;
-    }
-    const float *q = a.q + (size_t)i * a.ldq + (size_t)h * HD;
-    for (int d = lane; d < HD; d += 32) qs[w][d] = q[d] * a.scale;
-    __syncwarp();
-    float m = -INFINITY, l = 0.0f, o[HD / 32];
+    const Kv8Req rq = kv8_req(a, lo);
+    if (i - rq.row0 < 0 || i - rq.row0 >= rq.T) return;
+    int SL;
+    const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
+    if (ns == 1) return;
+    // only the splits that begin at or before the row's own token hold anything
+    const int live = min(ns, (rq.pos + (i - rq.row0)) / SL + 1);
+    const float *rec = a.part + ((size_t)i * a.H + h) * a.S * (HD + 4);
+    float M = -INFINITY, L = 0.0f, o[HD / 32];
+#pragma unroll
     for (int d = 0; d < HD / 32; d++) o[d] = 0.0f;
-    const uint8_t *kc = (const uint8_t *)a.kv.k, *vc = (const uint8_t *)a.kv.v;
-    for (long long j0 = 0; j0 <= last; j0 += 32) {
-        const long long j = j0 + lane;
-        float s = -INFINITY, vs = 0.0f;
-        size_t at = 0;
-        if (j <= last) {
-            const int b = a.table[(size_t)r * a.max_blocks + j / bs];
-            if (b >= 0 && b < a.kv.n_blocks) {
-                const size_t bh = (size_t)b * KH + kvh;
-                at = (bh * bs + j % bs) * HD;
-                vs = a.kv.v_scale[bh];
-                float dot = 0.0f;
-                for (int d = 0; d < HD; d++) dot = fmaf(qs[w][d], kv8_value<TYPE>(kc[at + d]), dot);
-                s = dot * a.kv.k_scale[bh];
-            } else {
-                vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+    if (rq.pos + (i - rq.row0) >= 0) {
+        for (int s = 0; s < live; s++) M = fmaxf(M, rec[(size_t)s * (HD + 4)]);
+#pragma unroll 4
+        for (int s = 0; s < live; s++) {
+            const float2 ml = *reinterpret_cast<const float2 *>(rec + (size_t)s * (HD + 4));
+            const float e = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+            L = fmaf(e, ml.y, L);
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++) {
+                const float x = rec[(size_t)s * (HD + 4) + 4 + d * 32 + lane];
+                o[d] = fmaf(e, e != 0.0f ? x : 0.0f, o[d]);
             }
         }
-        const float mn = fmaxf(m, warp_max(s));
-        if (mn == -INFINITY) continue;
-        const float c = expf(m - mn), e = s == -INFINITY ? 0.0f : expf(s - mn);
-        l = l * c + warp_sum(e);
-        for (int d = 0; d < HD / 32; d++) o[d] *= c;
-        m = mn;
-        for (int jj = 0; jj < 32; jj++) {
-            const float ej = __shfl_sync(0xffffffffu, e, jj) * __shfl_sync(0xffffffffu, vs, jj);
-            const size_t aj = __shfl_sync(0xffffffffu, at, jj);
-            if (ej == 0.0f) continue;
-            for (int d = 0; d < HD / 32; d++) o[d] = fmaf(ej, kv8_value<TYPE>(vc[aj + d * 32 + lane]), o[d]);
-        }
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
     float *out = a.out + (size_t)i * a.ldo + (size_t)h * HD;
+#pragma unroll
     for (int d = 0; d < HD / 32; d++) out[d * 32 + lane] = o[d] * inv;
-}
-
-typedef void (*attn_rows_t)(const Kv8AttnArgs);
-template <int TYPE>
-static attn_rows_t attn_rows_kernel(int hd) {
-    switch (hd) {
-        case 32: return k_kv8_attn_rows<TYPE, 32>;
-        case 64: return k_kv8_attn_rows<TYPE, 64>;
-        case 96: return k_kv8_attn_rows<TYPE, 96>;
-        default: return k_kv8_attn_rows<TYPE, 128>;
-    }
 }
 
 static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
@@ -102,7 +501,7 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
         return -4;
     }
     if (n_req < 1 || n_req > VXC_KV8_MAX_REQ || n_rows < 0 || n_rows > VXC_KV8_MAX_ROWS || max_new < 1 ||
-        max_blocks < 1 || (long long)max_blocks * kv->block_size > INT_MAX) {
+        max_blocks < 1 || (long long)max_blocks * kv->block_size > KV8_MAX_TOKENS) {
         vxc_set_error("vxc_kv8_attn: %d requests, %d rows (%d of one request), %d blocks per request", n_req, n_rows,
                       max_new, max_blocks);
         return -4;
@@ -110,10 +509,60 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
     return 0;
 }
 
+// How a call is cut: queries per CTA and splits.
+struct AttnPlan {
+    int nq;        // queries per chunk (k_kv8_attn_few)
+    int chunks;    // chunks per (request, kv head) at most
+    int S, sl_min;
+};
+#define ATTN_SL_MIN 256
+
+static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
+    AttnPlan p;
+    const int G = n_heads / kv->n_kv_heads;
+    const long long most = (long long)(max_new < n_rows ? max_new : n_rows) * G;   // queries of a request
+    p.nq = most <= 8 ? 8 : 16;
+    p.chunks = (int)((most + p.nq - 1) / p.nq);
+    // splits: two rounds of CTAs on the GPU when every request has a full table
+    const long long units = (long long)n_req * kv->n_kv_heads * p.chunks;
+    const long long tokens = (long long)max_blocks * kv->block_size;
+    long long S = (2 * 148 * 3 + units - 1) / units;
+    const long long need = (tokens + ATTN_SL_MIN - 1) / ATTN_SL_MIN;
+    if (S > need) S = need;
+    if (S > 64) S = 64;
+    // a tensor core's sums lose up to an ulp per step: 8192 tokens are 128 steps per warp, 5e-6 at most
+    if (S < (tokens + 8191) / 8192) S = (tokens + 8191) / 8192;
+    p.S = (int)(S < 1 ? 1 : S);
+    p.sl_min = ATTN_SL_MIN;
+    return p;
+}
+
 extern "C" size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new,
                                                int max_blocks) {
     if (attn_check(kv, n_heads, n_req, n_rows, max_new, max_blocks)) return 0;
-    return 0;
+    const AttnPlan p = attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks);
+    return p.S > 1 ? (size_t)n_rows * n_heads * p.S * (kv->head_dim + 4) * sizeof(float) : 0;
+}
+
+typedef void (*attn_kernel_t)(const Kv8AttnArgs);
+template <int TYPE, int HD>
+static attn_kernel_t few_kernel(int nq) { return nq == 8 ? k_kv8_attn_few<TYPE, HD, 8> : k_kv8_attn_few<TYPE, HD, 16>; }
+template <int TYPE>
+static attn_kernel_t few_kernel(int hd, int nq) {
+    switch (hd) {
+        case 32: return few_kernel<TYPE, 32>(nq);
+        case 64: return few_kernel<TYPE, 64>(nq);
+        case 96: return few_kernel<TYPE, 96>(nq);
+        default: return few_kernel<TYPE, 128>(nq);
+    }
+}
+static attn_kernel_t join_kernel(int hd) {
+    switch (hd) {
+        case 32: return k_kv8_attn_join<32>;
+        case 64: return k_kv8_attn_join<64>;
+        case 96: return k_kv8_attn_join<96>;
+        default: return k_kv8_attn_join<128>;
+    }
 }
 
 extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, int n_heads, float scale,
@@ -132,14 +581,24 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
         vxc_set_error("vxc_kv8_attn: scale is not finite");
         return -4;
     }
+    const AttnPlan p = attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks);
+    const size_t need = vxc_kv8_attn_workspace_bytes(kv, n_heads, n_req, n_rows, max_new, max_blocks);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) {
+        vxc_set_error("vxc_kv8_attn: workspace of %zu bytes needed (16-byte aligned)", need);
+        return -4;
+    }
     if (int rc = vxc_require_device()) return rc;
     if (n_rows == 0) return 0;
-    (void)workspace;
-    (void)workspace_bytes;
-    Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, n_req, n_rows, max_new, out, ldo,
-                     vxc_device_error_ptr()};
-    attn_rows_t f = kv->type == VXC_KV8_INT8 ? attn_rows_kernel<VXC_KV8_INT8>(kv->head_dim)
-                                             : attn_rows_kernel<VXC_KV8_E4M3>(kv->head_dim);
-    VXC_CUDA_OK(kv8_launch(f, dim3(n_rows, (n_heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, 1, a));
+    const int hd = kv->head_dim;
+    const Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, n_req, n_rows, max_new,
+                           out, ldo, (float *)workspace, p.S, p.sl_min, vxc_device_error_ptr()};
+    attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
+    size_t smem = (size_t)4 * FEW_STAGES * (hd * 32 + 16);
+    const size_t join = (size_t)4 * p.nq * (hd + 6) * sizeof(float);
+    if (smem < join) smem = join;
+    VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
+    VXC_CUDA_OK(kv8_launch(f, dim3(kv->n_kv_heads * p.chunks, p.S, n_req), dim3(128), smem, (cudaStream_t)stream, 1, a));
+    if (p.S > 1)
+        VXC_CUDA_OK(kv8_launch(join_kernel(hd), dim3(n_rows, (n_heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, 1, a));
     return 0;
 }
