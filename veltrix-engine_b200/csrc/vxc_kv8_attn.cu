@@ -1,25 +1,7 @@
 // vxc_kv8_attn.cu — causal attention over the paged 8-bit KV cache
 // (reference src/model.c:299-338, over its fp32 cache).
 //   out_i,h = sum_j softmax_j(scale q_i,h . k_j) v_j,  j <= position of row i
-#include "vxc_kv8.cuh"
-
-struct Kv8AttnArgs {
-    vxc_kv8 kv;
-    const float *q;
-    long long ldq;
-    int H;
-    float scale;
-    const int *table;
-    int max_blocks;
-    const int *row0;    // [n_req + 1]
-    const int *pos;     // [n_req]
-    int n_req, n_rows, max_new;
-    float *out;
-    long long ldo;
-    float *part;        // records of the splits
-    int S, sl_min;      // splits per request at most, tokens per split at least
-    unsigned int *err;
-};
+#include "vxc_kv8_attn.cuh"
 
 // ---------------------------------------------------------------------------
 // Few queries per kv head (decode and small verify steps): split over the
@@ -38,9 +20,9 @@ struct Kv8AttnArgs {
 //     their two sums are added: one instruction does both products.
 //   NQ = 16: two instructions into the same sums, hi and lo.
 // Layouts.  The sum over the head dim may go in any order, so lane t of a quad
-// takes the pieces of a K row that it can load as whole words (kv8_k_at), and
+// takes the pieces of a K row that it can load as whole words (Kv8Piece::k_at), and
 // the query's fragment is loaded in the same order.  Likewise the output's
-// columns: lane group g takes pieces of a V row (kv8_v_at).  So every byte goes
+// columns: lane group g takes pieces of a V row (Kv8Piece::v_at).  So every byte goes
 // by cp.async to the ring slot of the lane that uses it, and back from there
 // without a bank conflict; no lane reads another's bytes and the ring needs no
 // barrier.  Scores come out where the weights' fragment wants them: lane (g, t)
@@ -54,8 +36,6 @@ struct Kv8AttnArgs {
 // Tokens behind the request's last one and blocks outside the cache are read
 // as zeros (cp.async's zero fill), so nothing of theirs reaches a product.
 // ---------------------------------------------------------------------------
-#define KV8_HEAD 10.0f   // weights up to 2^(10 + 5): in fp16's range with 2^-34 of the largest as last place
-#define KV8_LAG 5.0f
 #define FEW_STAGES 4     // 16-token tiles in flight per warp
 
 // Bytes that one cp.async brings, and the offset of piece c in a row.
@@ -67,89 +47,11 @@ struct Kv8Piece {
     static __device__ __forceinline__ int v_at(int c, int g) { return c * 8 * V + g * V; }
 };
 
-template <int N>
-__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void *src, bool have) {
-    const int n = have ? N : 0;
-    if (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// a, b -> half2 of their fp16 roundings, and half2 of what is left
-__device__ __forceinline__ uint32_t split_h2(float a, float b, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// Four codes -> two half2, bytes (0, 1) and (2, 3).  int8: the byte with its
-// sign bit flipped is the low byte of the half 1024 + 128 + code.
-template <int TYPE>
-__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &h01, uint32_t &h23) {
-    if (TYPE == VXC_KV8_INT8) {
-        const uint32_t x = w ^ 0x80808080u;
-        uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        const __half2 ha = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
-        h01 = *reinterpret_cast<const uint32_t *>(&ha);
-        h23 = *reinterpret_cast<const uint32_t *>(&hb);
-    } else {
-        h01 = kv8_e4m3x2_h2((uint16_t)(w & 0xFFFFu));
-        h23 = kv8_e4m3x2_h2((uint16_t)(w >> 16));
-    }
-}
-
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// A request's rows and tokens as the call's arguments and arrays allow them.
-struct Kv8Req {
-    int row0, T;     // first row; rows (clamped to n_rows, max_new and the table)
-    int pos;         // position of the first row
-    int kvlen;       // tokens the last row sees (0: none)
-    bool over;       // something was clamped
-};
-__device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
-    Kv8Req q;
-    const int r0 = a.row0[r], r1 = a.row0[r + 1];
-    q.pos = a.pos[r];
-    q.row0 = max(r0, 0);
-    long long T = (long long)r1 - r0;
-    const long long cap = (long long)a.max_blocks * a.kv.block_size;
-    const long long most = min(min((long long)a.max_new, (long long)a.n_rows - q.row0), cap - q.pos);
-    q.over = r0 < 0 || T > most;
-    T = r0 < 0 ? 0 : min(T, most);
-    q.T = (int)max(T, 0ll);
-    q.kvlen = q.T > 0 ? max(q.pos + q.T, 0) : 0;
-    return q;
-}
-
-// Splits of a request: enough for SL_min tokens each, at most S.
-__device__ __forceinline__ int kv8_splits(int kvlen, int sl_min, int S, int &SL) {
-    const int want = min(max((kvlen + sl_min - 1) / sl_min, 1), S);
-    SL = ((kvlen + want - 1) / want + 63) & ~63;
-    return SL > 0 ? (kvlen + SL - 1) / SL : 1;
 }
 
 // Records of the splits: [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum
@@ -509,31 +411,45 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
     return 0;
 }
 
-// How a call is cut: queries per CTA and splits.
+// How a call is cut: kernel, queries per CTA and splits.
 struct AttnPlan {
-    int nq;        // queries per chunk (k_kv8_attn_few)
-    int chunks;    // chunks per (request, kv head) at most
+    int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), KV8_TILE_Q (k_kv8_attn_many)
+    int chunks;    // chunks per (request, kv head) at most, or tiles of all requests
     int S, sl_min;
 };
-#define ATTN_SL_MIN 256
+#ifndef ATTN_FEW_MAX
+#define ATTN_FEW_MAX 16   // queries of a request and kv head up to which k_kv8_attn_few is used
+#endif
 
 static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
     AttnPlan p;
     const int G = n_heads / kv->n_kv_heads;
     const long long most = (long long)(max_new < n_rows ? max_new : n_rows) * G;   // queries of a request
-    p.nq = most <= 8 ? 8 : 16;
-    p.chunks = (int)((most + p.nq - 1) / p.nq);
-    // splits: two rounds of CTAs on the GPU when every request has a full table
-    const long long units = (long long)n_req * kv->n_kv_heads * p.chunks;
     const long long tokens = (long long)max_blocks * kv->block_size;
-    long long S = (2 * 148 * 3 + units - 1) / units;
-    const long long need = (tokens + ATTN_SL_MIN - 1) / ATTN_SL_MIN;
+    long long units, S;
+    if (most <= ATTN_FEW_MAX) {
+        p.nq = most <= 8 ? 8 : 16;
+        p.chunks = (int)((most + p.nq - 1) / p.nq);
+        p.sl_min = 256;
+        // two rounds of CTAs on the GPU when every request has a full table
+        units = (long long)n_req * kv->n_kv_heads * (p.chunks > 0 ? p.chunks : 1);
+        S = (2 * 148 * 3 + units - 1) / units;
+    } else {
+        p.nq = KV8_TILE_Q;
+        const long long full = (long long)n_rows * G / KV8_TILE_Q;
+        p.chunks = (int)(full + n_req);
+        p.sl_min = 512;
+        const long long busy = n_req < n_rows ? n_req : n_rows;
+        units = (full > busy ? full : busy) * kv->n_kv_heads;
+        S = units >= 2 * 148 ? 1 : (3 * 148 + units - 1) / units;
+    }
+    const long long need = (tokens + p.sl_min - 1) / p.sl_min;
     if (S > need) S = need;
     if (S > 64) S = 64;
-    // a tensor core's sums lose up to an ulp per step: 8192 tokens are 128 steps per warp, 5e-6 at most
-    if (S < (tokens + 8191) / 8192) S = (tokens + 8191) / 8192;
+    // k_kv8_attn_few: a tensor core's sums lose up to an ulp per step: 8192 tokens are 128 steps per
+    // warp, 5e-6 at most
+    if (p.nq < KV8_TILE_Q && S < (tokens + 8191) / 8192) S = (tokens + 8191) / 8192;
     p.S = (int)(S < 1 ? 1 : S);
-    p.sl_min = ATTN_SL_MIN;
     return p;
 }
 
@@ -592,12 +508,16 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
     const int hd = kv->head_dim;
     const Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, n_req, n_rows, max_new,
                            out, ldo, (float *)workspace, p.S, p.sl_min, vxc_device_error_ptr()};
-    attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
-    size_t smem = (size_t)4 * FEW_STAGES * (hd * 32 + 16);
-    const size_t join = (size_t)4 * p.nq * (hd + 6) * sizeof(float);
-    if (smem < join) smem = join;
-    VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
-    VXC_CUDA_OK(kv8_launch(f, dim3(kv->n_kv_heads * p.chunks, p.S, n_req), dim3(128), smem, (cudaStream_t)stream, 1, a));
+    if (p.nq == KV8_TILE_Q) {
+        VXC_CUDA_OK(kv8_attn_many(a, p.chunks, (cudaStream_t)stream));
+    } else {
+        attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
+        size_t smem = (size_t)4 * FEW_STAGES * (hd * 32 + 16);
+        const size_t join = (size_t)4 * p.nq * (hd + 6) * sizeof(float);
+        if (smem < join) smem = join;
+        VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
+        VXC_CUDA_OK(kv8_launch(f, dim3(kv->n_kv_heads * p.chunks, p.S, n_req), dim3(128), smem, (cudaStream_t)stream, 1, a));
+    }
     if (p.S > 1)
         VXC_CUDA_OK(kv8_launch(join_kernel(hd), dim3(n_rows, (n_heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, 1, a));
     return 0;

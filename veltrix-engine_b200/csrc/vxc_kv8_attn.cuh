@@ -1,0 +1,109 @@
+// vxc_kv8_attn.cuh — what the attention kernels over the paged 8-bit KV cache
+// share: their arguments, a request's bounds, and the arithmetic of codes,
+// queries and weights.
+#pragma once
+#include "vxc_kv8.cuh"
+
+struct Kv8AttnArgs {
+    vxc_kv8 kv;
+    const float *q;
+    long long ldq;
+    int H;
+    float scale;
+    const int *table;
+    int max_blocks;
+    const int *row0;    // [n_req + 1]
+    const int *pos;     // [n_req]
+    int n_req, n_rows, max_new;
+    float *out;
+    long long ldo;
+    float *part;        // records of the splits
+    int S, sl_min;      // splits per request at most, tokens per split at least
+    unsigned int *err;
+};
+
+#define KV8_HEAD 10.0f   // weights up to 2^(10 + 5): in fp16's range with 2^-34 of the largest as last place
+#define KV8_LAG 5.0f
+
+template <int N>
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void *src, bool have) {
+    const int n = have ? N : 0;
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// a, b -> half2 of their fp16 roundings, and half2 of what is left
+__device__ __forceinline__ uint32_t split_h2(float a, float b, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Four codes -> two half2, bytes (0, 1) and (2, 3).  int8: the byte with its
+// sign bit flipped is the low byte of the half 1024 + 128 + code.
+template <int TYPE>
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &h01, uint32_t &h23) {
+    if (TYPE == VXC_KV8_INT8) {
+        const uint32_t x = w ^ 0x80808080u;
+        uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const __half2 ha = __hsub2(*reinterpret_cast<__half2 *>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2 *>(&b), bias);
+        h01 = *reinterpret_cast<const uint32_t *>(&ha);
+        h23 = *reinterpret_cast<const uint32_t *>(&hb);
+    } else {
+        h01 = kv8_e4m3x2_h2((uint16_t)(w & 0xFFFFu));
+        h23 = kv8_e4m3x2_h2((uint16_t)(w >> 16));
+    }
+}
+
+// A request's rows and tokens as the call's arguments and arrays allow them.
+struct Kv8Req {
+    int row0, T;     // first row; rows (clamped to n_rows, max_new and the table)
+    int pos;         // position of the first row
+    int kvlen;       // tokens the last row sees (0: none)
+    bool over;       // something was clamped
+};
+__device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
+    Kv8Req q;
+    const int r0 = a.row0[r], r1 = a.row0[r + 1];
+    q.pos = a.pos[r];
+    q.row0 = max(r0, 0);
+    long long T = (long long)r1 - r0;
+    const long long cap = (long long)a.max_blocks * a.kv.block_size;
+    const long long most = min(min((long long)a.max_new, (long long)a.n_rows - q.row0), cap - q.pos);
+    q.over = r0 < 0 || T > most;
+    T = r0 < 0 ? 0 : min(T, most);
+    q.T = (int)max(T, 0ll);
+    q.kvlen = q.T > 0 ? max(q.pos + q.T, 0) : 0;
+    return q;
+}
+
+// Splits of a request: enough for SL_min tokens each, at most S.
+__device__ __forceinline__ int kv8_splits(int kvlen, int sl_min, int S, int &SL) {
+    const int want = min(max((kvlen + sl_min - 1) / sl_min, 1), S);
+    SL = ((kvlen + want - 1) / want + 127) & ~127;
+    return SL > 0 ? (kvlen + SL - 1) / SL : 1;
+}
+
+// Many queries per kv head (vxc_kv8_attn_many.cu): launch over at most `tiles`
+// tiles of KV8_TILE_Q queries.
+#define KV8_TILE_Q 128
+cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tiles, cudaStream_t st);
