@@ -18,14 +18,16 @@
 // (in and out), as fp16 (in) and as operands: as much time again.  (Q from
 // shared memory added half of that: hence in TMEM.)
 //
-// Roles (512 threads, one CTA per SM):
-//   warps 0-3    loaders: cp.async 8-bit rows into slots of each thread's own
+// Roles (640 threads, one CTA per SM):
+//   warps 0-7    loaders: cp.async 8-bit rows into slots of each thread's own
 //                (MN_AHEAD pieces ahead), convert, store fp16 core matrices
-//   warps 4-7 and 8-11   softmax groups A and B, thread = query: even and odd
-//                tiles, each with its own S / P buffer, maxima, sum and output
-//                registers
-//   warp 12      issues S of tile j + 2; warp 13 issues P V of tile j
-//   warp 14      block table and scales of the coming tiles
+//   warps 8-15   softmax, two threads per query: warps 8-11 have tokens 0-63 of
+//                a tile and the first half of the output columns, warps 12-15
+//                the others; they exchange their maxima through shared memory.
+//                Weights of tile j first, then O of tile j - 1 is added, so its
+//                product runs beside them
+//   warp 16      issues S of tile j + 2; warp 17 issues P V of tile j
+//   warp 18      block table and scales of the coming tiles
 // TMEM: two buffers of 128 columns for S / P, 128 for O, 128 for Q.
 // K and V tiles have two slots each.  K as [head dim chunk][token] x 16 bytes
 // is K-major, V in the same layout is MN-major; chunks are 2064 bytes apart, so
@@ -34,7 +36,8 @@
 // role leaves its loop, and TMEM is freed after the issued work has ended.
 #include "vxc_kv8_attn.cuh"
 
-#define MN_THREADS 512
+#define MN_LOADERS 256         // warps 0-7
+#define MN_THREADS (MN_LOADERS + 256 + 128)
 #define MN_CHUNK 2064          // bytes between 8-column chunks of a 128-row fp16 tile
 #define MN_PAGES 8             // tiles whose blocks and scales are held
 #define MN_AHEAD 4             // K or V pieces of raw bytes in flight
@@ -59,13 +62,42 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
         : "memory");
 }
 
+// Two floats at once.
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
                  "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
-// The two softmax groups only.
+// mbar_wait behind a first look without a suspend hint: most phases are complete when asked for.
+__device__ __forceinline__ bool mn_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned int *err,
+                                        unsigned int code) {
+    return mbar_try(bar, parity) || mbar_wait(bar, parity, abort_flag, err, code);
+}
+
+// The softmax warps only.
 __device__ __forceinline__ void mn_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <int TYPE, int HD>
@@ -74,7 +106,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ __align__(8) uint64_t bars[18 + 2 * MN_PAGES];
     __shared__ long long page_at[MN_PAGES][8];     // byte offset of a 16-token group in the cache; -1 none, -2 bad block
-    __shared__ float page_ks[MN_PAGES][8], page_vs[MN_PAGES][8], page_lv[MN_PAGES][8];
+    __shared__ __align__(16) float page_ks[MN_PAGES][8], page_vs[MN_PAGES][8], page_lv[MN_PAGES][8];
+    __shared__ float2 red[2][2][128];              // [tile parity][half][query]: maxima of half a tile
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -108,75 +141,40 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     const int nt = p1 > p0 ? (p1 - p0 + 127) >> 7 : 0;
 
     const uint32_t bar0 = smem_u32(bars);
-    auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (128 loaders)
-    auto kempty = [&](int s) { return bar0 + 8u * (2 + s); };      // S product read it
-    auto vfull = [&](int s) { return bar0 + 8u * (4 + s); };
-    auto vempty = [&](int s) { return bar0 + 8u * (6 + s); };
-    auto sfull = [&](int g) { return bar0 + 8u * (8 + g); };       // S product of group g's tile done
-    auto pfull = [&](int g) { return bar0 + 8u * (10 + g); };      // its weights stored (128 threads)
-    auto ofull = [&](int g) { return bar0 + 8u * (12 + g); };      // its P V product done
-    auto oempty = [&](int g) { return bar0 + 8u * (14 + g); };     // group g has read O
+    auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (loaders)
+    auto vfull = [&](int s) { return bar0 + 8u * (2 + s); };
+    auto sfull = [&](int b) { return bar0 + 8u * (8 + b); };       // S product of a tile in buffer b done: its K slot is free
+    auto pfull = [&](int b) { return bar0 + 8u * (10 + b); };      // its weights stored (256 threads)
+    auto ofull = [&](int b) { return bar0 + 8u * (12 + b); };      // its P V product done: its V slot is free
+    const uint32_t oempty = bar0 + 8u * 14, qfull = bar0 + 8u * 15;   // O read; queries stored (256 threads)
     auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks and scales of a tile (8 lanes)
     auto gempty = [&](int s) { return bar0 + 8u * (26 + s); };     // loaders (after V) and the softmax group are done with them
     if (tid == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(kfull(s), 128), mbar_init(kempty(s), 1), mbar_init(vfull(s), 128), mbar_init(vempty(s), 1);
-            mbar_init(sfull(s), 1), mbar_init(pfull(s), 128), mbar_init(ofull(s), 1), mbar_init(oempty(s), 128);
+            mbar_init(kfull(s), MN_LOADERS), mbar_init(vfull(s), MN_LOADERS);
+            mbar_init(sfull(s), 1), mbar_init(pfull(s), 256), mbar_init(ofull(s), 1);
             mbar_init(bar0 + 8u * (16 + s), 1);   // an issuer's last work, after an abort
         }
-        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 8), mbar_init(gempty(s), 256);
+        mbar_init(oempty, 256), mbar_init(qfull, 256);
+        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 8), mbar_init(gempty(s), MN_LOADERS + 256);
         abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 12) tmem_alloc(smem_u32(&tmem_slot), 512u);
+    if (warp == 16) tmem_alloc(smem_u32(&tmem_slot), 512u);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot, t_o = tmem + 256, t_q = tmem + 384;   // Q: hi in HD / 2 columns, lo 64 columns on
-    float f = 0.0f;   // softmax threads: factor of the query's scores
-    if (warp >= 4 && warp < 12) {
-        // queries into TMEM, thread = query, groups A and B half of the head dim each
-        const int q = q0 + (tid & 127), half = (warp >> 2) - 1;
-        const float4 *src = reinterpret_cast<const float4 *>(a.q + (size_t)(rq.row0 + (q < nq ? q / G : 0)) * a.ldq +
-                                                             (size_t)(kvh * G + q % G) * HD);
-        float mx = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < HD / 4; i++) {
-            const float4 v = src[i];
-            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-        // the row's largest element into [2^13, 2^14); a negative scale goes into the queries, since
-        // the maxima are taken before the factor is applied
-        const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
-        const float up = copysignf(__uint_as_float((uint32_t)(267 - ex) << 23), a.scale);
-        f = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 13) << 23);
-        const uint32_t dst = t_q + ((uint32_t)((warp & 3) * 32) << 16) + half * (HD / 4);
-#pragma unroll 1
-        for (int c = 0; c < HD / 16; c += 2) {   // 8 columns of hi and of lo from 4 float4
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 v = src[half * (HD / 8) + (c / 2) * 4 + i];
-                hi[2 * i] = split_h2(v.x * up, v.y * up, lo[2 * i]);
-                hi[2 * i + 1] = split_h2(v.z * up, v.w * up, lo[2 * i + 1]);
-            }
-            tmem_st8(dst + 4 * c, hi);
-            tmem_st8(dst + 64 + 4 * c, lo);
-        }
-        tmem_wait_st();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     volatile int *abortp = &abort_flag;
     unsigned int *err = a.err;
     const uint32_t smb = smem_u32(sm);
 
-    if (warp < 4) {
+    if (warp < MN_LOADERS / 32) {
         // ------------------------------ loaders ------------------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // pieces in the order K0, K1, V0, K2, V1, ..., V(nt - 1); 16-byte units, TPR threads a row
-        constexpr int TPR = HD == 96 ? 8 : HD / 16, RP = 128 / TPR;
+        constexpr int TPR = HD == 96 ? 8 : HD / 16, RP = MN_LOADERS / TPR, NP = 128 / RP;   // rows a pass, passes
+        static_assert(RP % 16 == 0 && NP >= 1, "whole groups of 16 tokens a pass");
         const int c = tid % TPR, tr = tid / TPR;
         const bool on = c < HD / 16;
         const uint32_t raw = smb + M::RAW + tid * 16;
@@ -187,17 +185,17 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             if (i < np) {
                 const int j = tile_of(i), e = j % MN_PAGES;
                 const bool isv = is_v(i);
-                if (!mbar_wait(gfull(e), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA)) return false;
+                if (!mn_wait(gfull(e), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA)) return false;
                 const uint8_t *base = (const uint8_t *)(isv ? a.kv.v : a.kv.k);
                 const uint8_t *src = base + (tr & 15) * HD + c * 16;
                 const uint32_t dst = raw + (i % MN_AHEAD) * M::PIECE;
                 const int live = rq.kvlen - (p0 + 128 * j);
                 if (on) {
 #pragma unroll
-                    for (int k = 0; k < TPR; k++) {
+                    for (int k = 0; k < NP; k++) {
                         const long long at = page_at[e][k * (RP / 16) + (tr >> 4)];
                         const bool have = at >= 0 && k * RP + tr < live;
-                        cp_async_zfill<16>(dst + k * 2048, have ? src + at : base, have);
+                        cp_async_zfill<16>(dst + k * (MN_LOADERS * 16), have ? src + at : base, have);
                     }
                 }
                 if (isv) mbar_arrive(gempty(e));
@@ -212,7 +210,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             const int j = tile_of(i), s = j & 1;
             const bool isv = is_v(i);
             cp_wait<MN_AHEAD - 1>();
-            if (j >= 2) ok = mbar_wait(isv ? vempty(s) : kempty(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            if (j >= 2) ok = mn_wait(isv ? ofull(s) : sfull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
             if (!ok) break;
             unsigned char *dst = sm + (isv ? M::V : M::K) + s * M::TILE + 2 * c * MN_CHUNK + tr * 16;
             const unsigned char *src = sm + M::RAW + tid * 16 + (i % MN_AHEAD) * M::PIECE;
@@ -222,8 +220,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             unsigned char *d0 = dst + (swap ? MN_CHUNK : 0), *d1 = dst + (swap ? 0 : MN_CHUNK);
             if (on) {
 #pragma unroll
-                for (int k = 0; k < TPR; k++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(src + k * 2048);
+                for (int k = 0; k < NP; k++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(src + k * (MN_LOADERS * 16));
                     uint4 h0, h1;
                     codes_h2<TYPE>(swap ? w.z : w.x, h0.x, h0.y);
                     codes_h2<TYPE>(swap ? w.w : w.y, h0.z, h0.w);
@@ -239,61 +237,125 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         }
         cp_wait<0>();
         __syncwarp();
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");   // what the block was launched with, for the code behind the roles
-    } else if (warp < 12) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");   // what the block was launched with, for the code behind the roles
+    } else if (warp < MN_LOADERS / 32 + 8) {
         // ------------------------------ softmax ------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        const int grp = (warp >> 2) - 1, row = tid & 127;
-        float m = -INFINITY, mv = -INFINITY, l = 0.0f;
-        float acc[HD];
-#pragma unroll
-        for (int d = 0; d < HD; d++) acc[d] = 0.0f;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        constexpr int HC = HD / 2;   // elements of a query, columns of O per thread
+        const int half = (warp >> 2) - MN_LOADERS / 128, row = tid & 127;
         const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + tl + 128 * grp;
         const int q = q0 + row;
+        float f;   // factor of the query's scores
+        {
+            // half a query into TMEM
+            float4 v[HC / 4];
+            const float4 *src = reinterpret_cast<const float4 *>(a.q + (size_t)(rq.row0 + (q < nq ? q / G : 0)) * a.ldq +
+                                                                 (size_t)(kvh * G + q % G) * HD + half * HC);
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HC / 4; i++) v[i] = src[i];
+#pragma unroll
+            for (int i = 0; i < HC / 4; i++)
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+            red[1][half][row].x = mx;
+            mn_group_sync();
+            mx = fmaxf(mx, red[1][half ^ 1][row].x);
+            // the row's largest element into [2^13, 2^14); a negative scale goes into the queries, since
+            // the maxima are taken before the factor is applied
+            const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
+            const float up = copysignf(__uint_as_float((uint32_t)(267 - ex) << 23), a.scale);
+            f = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 13) << 23);
+#pragma unroll
+            for (int c = 0; c < HC / 16; c++) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 x = v[4 * c + i];
+                    hi[2 * i] = split_h2(x.x * up, x.y * up, lo[2 * i]);
+                    hi[2 * i + 1] = split_h2(x.z * up, x.w * up, lo[2 * i + 1]);
+                }
+                tmem_st8(t_q + tl + half * (HC / 2) + 8 * c, hi);
+                tmem_st8(t_q + tl + 64 + half * (HC / 2) + 8 * c, lo);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(qfull);
+        }
+        float m = -INFINITY, mv = -INFINITY, l = 0.0f;
+        float acc[HC];
+#pragma unroll
+        for (int d = 0; d < HC; d++) acc[d] = 0.0f;
         const int lim = q < nq ? rq.pos + q / G : -1;
-#pragma unroll 1
-        for (int j = grp; j < nt; j += 2) {
-            const int e = j % MN_PAGES;
-            bool ok = mbar_wait(gfull(e), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
-            ok = ok && mbar_wait(sfull(grp), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-            if (!__all_sync(0xffffffffu, ok)) break;
+        // adds O of tile j to the registers
+        auto drain = [&](int j) -> bool {
+            const bool ok = mn_wait(ofull(j & 1), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            if (!__all_sync(0xffffffffu, ok)) return false;
             tc_fence_after();
-            const int t0 = p0 + 128 * j;
-            // bit c: group c of 16 tokens lies in a block outside the cache
-            const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && page_at[e][lane & 7] == -2);
-            const bool whole = __all_sync(0xffffffffu, lim >= t0 + 127) && bad == 0;
-            // visible tokens of group c: the low bits of a mask
-            auto mask = [&](int c) -> uint32_t {
-                const int n = lim - (t0 + 16 * c) + 1;
-                return ((bad >> c) & 1u) || n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
-            };
-            float mx = -INFINITY, mxv = -INFINITY;
+            uint32_t v[HC];
+#pragma unroll
+            for (int c = 0; c < HC / 16; c++) tmem_ld16(t_o + tl + half * HC + 16 * c, v + 16 * c);
+            tmem_wait_ld();
+            tmem_pin<HC>(v);
+#pragma unroll
+            for (int d = 0; d < HC; d++) acc[d] += __uint_as_float(v[d]);
+            tc_fence_before();
+            mbar_arrive(oempty);
+            return true;
+        };
+        bool ok = true;
 #pragma unroll 1
-            for (int c2 = 0; c2 < 4; c2++) {
-                uint32_t v[32];
-                tmem_ld32(t_s + 32 * c2, v);
-                const float2 ks = *reinterpret_cast<const float2 *>(&page_ks[e][2 * c2]);
-                const float2 lv = *reinterpret_cast<const float2 *>(&page_lv[e][2 * c2]);
-                tmem_wait_ld();
-                tmem_pin<32>(v);
-                if (!whole) {
-                    const uint32_t mk = mask(2 * c2) | mask(2 * c2 + 1) << 16;
+        for (int j = 0; j < nt; j++) {
+            const int e = j % MN_PAGES, b = j & 1;
+            const uint32_t t_s = tmem + tl + 128 * b + 64 * half;
+            // (S is there, so the loaders have seen the tile's blocks and scales, and so does this thread)
+            ok = ok && mn_wait(sfull(b), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            // (after a failed wait the scores are garbage; every warp leaves at the barrier below)
+            __syncwarp();
+            tc_fence_after();
+            uint32_t v[64];
+            tmem_ld32(t_s, v);
+            tmem_ld32(t_s + 32, v + 32);
+            const int t0 = p0 + 128 * j + 64 * half;
+            const float4 ks = *reinterpret_cast<const float4 *>(&page_ks[e][4 * half]);
+            const float4 vs = *reinterpret_cast<const float4 *>(&page_vs[e][4 * half]);
+            const float4 lv = *reinterpret_cast<const float4 *>(&page_lv[e][4 * half]);
+            const float fk[4] = {f * ks.x, f * ks.y, f * ks.z, f * ks.w};
+            // bit c: group c of 16 tokens lies in a block outside the cache
+            const uint32_t bad = __ballot_sync(0xffffffffu, lane < 4 && page_at[e][4 * half + (lane & 3)] == -2);
+            const bool whole = __all_sync(0xffffffffu, lim >= t0 + 63) && bad == 0;
+            tmem_wait_ld();
+            tmem_pin<64>(v);
+            if (!whole) {
 #pragma unroll
-                    for (int k = 0; k < 32; k++) v[k] = (mk >> k) & 1u ? v[k] : 0xFF800000u;   // -inf
+                for (int c = 0; c < 4; c++) {   // visible tokens of group c: the low bits of a mask
+                    const int n = lim - (t0 + 16 * c) + 1;
+                    const uint32_t mk = ((bad >> c) & 1u) || n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) v[16 * c + k] = (mk >> k) & 1u ? v[16 * c + k] : 0xFF800000u;   // -inf
                 }
-                float x[2];
+            }
+            float mx = -INFINITY, mxv = -INFINITY;
+            {
+                const float lvc[4] = {lv.x, lv.y, lv.z, lv.w};
+                float x[4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    x[h] = __uint_as_float(v[16 * h]);
+                for (int c = 0; c < 4; c++) {
+                    x[c] = __uint_as_float(v[16 * c]);
 #pragma unroll
-                    for (int k = 1; k < 16; k++) x[h] = fmaxf(x[h], __uint_as_float(v[16 * h + k]));
+                    for (int k = 1; k < 16; k++) x[c] = fmaxf(x[c], __uint_as_float(v[16 * c + k]));
+                    // (no visible token: -inf, also where the scale is 0)
+                    x[c] = x[c] == -INFINITY ? x[c] : x[c] * fk[c];
+                    mx = fmaxf(mx, x[c]);
+                    mxv = fmaxf(mxv, x[c] + lvc[c]);
                 }
-                // (no visible token: -inf, also where the scale is 0)
-                x[0] = x[0] == -INFINITY ? x[0] : x[0] * (f * ks.x);
-                x[1] = x[1] == -INFINITY ? x[1] : x[1] * (f * ks.y);
-                mx = fmaxf(mx, fmaxf(x[0], x[1]));
-                mxv = fmaxf(mxv, fmaxf(x[0] + lv.x, x[1] + lv.y));
+            }
+            red[b][half][row] = make_float2(mx, mxv);
+            ok = bar_and(1, 256, ok);   // the softmax warps go on together or not at all
+            if (!ok) break;
+            {
+                const float2 o = red[b][half ^ 1][row];
+                mx = fmaxf(mx, o.x);
+                mxv = fmaxf(mxv, o.y);
             }
             if (mx > m + KV8_LAG || (m == -INFINITY && mx > m)) {
                 l *= ex2(m - mx);   // 0 at first
@@ -304,107 +366,96 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 shrink = ex2(mv - mxv);
                 mv = mxv;
             }
-            if (__any_sync(0xffffffffu, shrink != 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < HD; d++) acc[d] *= shrink;
-            }
             const float mref = m == -INFINITY ? 0.0f : m;
             const float cv = ex2(fminf(mref - mv + KV8_HEAD, 120.0f));
-            float l2 = 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < 8; c++) {
-                uint32_t v[16], w[16];
-                tmem_ld16(t_s + 16 * c, v);
-                const float fk = f * page_ks[e][c], cw = page_vs[e][c] * cv;
-                tmem_wait_ld();
-                tmem_pin<16>(v);
+            const float cw[4] = {vs.x * cv, vs.y * cv, vs.z * cv, vs.w * cv};
+            const uint64_t nm = f2(-mref, -mref);
+            uint64_t sum = f2(0.0f, 0.0f);
 #pragma unroll
-                for (int k = 0; k < 16; k++) v[k] = __float_as_uint(ex2(fmaf(__uint_as_float(v[k]), fk, -mref)));
-                if (!whole) {
-                    const uint32_t mk = mask(c);
-#pragma unroll
-                    for (int k = 0; k < 16; k++) v[k] = (mk >> k) & 1u ? v[k] : 0u;
-                }
+            for (int c = 0; c < 4; c++) {
+                const uint64_t fk2 = f2(fk[c], fk[c]), cw2 = f2(cw[c], cw[c]);
+                uint32_t w[16];
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
-                    const float x = __uint_as_float(v[k]), y = __uint_as_float(v[k + 1]);
-                    l += x;
-                    l2 += y;
-                    w[k / 2] = split_h2(x * cw, y * cw, w[8 + k / 2]);
+                    float x, y;
+                    unf2(fma2(f2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])), fk2, nm), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    if (!whole) {   // -inf times a scale of 0
+                        x = v[16 * c + k] == 0xFF800000u ? 0.0f : x;
+                        y = v[16 * c + k + 1] == 0xFF800000u ? 0.0f : y;
+                    }
+                    const uint64_t p = f2(x, y);
+                    sum = add2(sum, p);
+                    float wx, wy;
+                    const uint64_t wt = mul2(p, cw2);
+                    unf2(wt, wx, wy);
+                    const __half2 h = __floats2half2_rn(wx, wy);
+                    const float2 hf = __half22float2(h);
+                    unf2(add2(wt, f2(-hf.x, -hf.y)), wx, wy);
+                    const __half2 lo = __floats2half2_rn(wx, wy);
+                    w[k / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                    w[8 + k / 2] = *reinterpret_cast<const uint32_t *>(&lo);
                 }
-                // hi in columns 0-7 of the group's 16, lo in 8-15: only this group's scores are replaced
+                // hi in columns 0-7 of the group's 16, lo in 8-15
                 tmem_st16(t_s + 16 * c, w);
             }
-            l += l2;
+            {
+                float x, y;
+                unf2(sum, x, y);
+                l += x + y;
+            }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(pfull(grp));
+            mbar_arrive(pfull(b));
             mbar_arrive(gempty(e));
-            ok = mbar_wait(ofull(grp), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc_fence_after();
+            if (j > 0) ok = drain(j - 1);
+            if (__any_sync(0xffffffffu, shrink != 1.0f)) {
 #pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-                uint32_t v[32];
-                tmem_ld32(t_o + tl + 32 * c, v);
-                tmem_wait_ld();
-                tmem_pin<32>(v);
-#pragma unroll
-                for (int d = 0; d < 32; d++) acc[32 * c + d] += __uint_as_float(v[d]);
+                for (int d = 0; d < HC; d++) acc[d] *= shrink;
             }
-            tc_fence_before();
-            mbar_arrive(oempty(grp));
         }
-        // join of the groups, outputs in units of 2^m.  Both groups have waited for their last
-        // P V product, so no product reads shared memory any more (after an abort one may, but
-        // then nothing is written).
+        if (ok && nt > 0) drain(nt - 1);
+        // The last P V product is done, so no product reads shared memory any more (after an abort one
+        // may, but then nothing is written).  Outputs in units of 2^m, through shared memory.
         float *so = reinterpret_cast<float *>(sm + M::K);     // [HD][129]
-        float *st = so + HD * 129;                            // [128][4]: group B's m and l, the result's M and L
-        const float back = mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f));
-#pragma unroll
-        for (int d = 0; d < HD; d++) acc[d] *= back;
+        float2 *st = reinterpret_cast<float2 *>(so + HD * 129);   // [2][128]: m, l of a query's halves
         mn_group_sync();
-        if (grp == 1) {
-#pragma unroll
-            for (int d = 0; d < HD; d++) so[d * 129 + row] = acc[d];
-            st[4 * row] = m;
-            st[4 * row + 1] = l;
-        }
+        st[128 * half + row] = make_float2(m, l);
         mn_group_sync();
-        if (grp == 0) {
-            const float m1 = st[4 * row], l1 = st[4 * row + 1], mm = fmaxf(m, m1);
-            const float e0 = m == -INFINITY ? 0.0f : ex2(m - mm), e1 = m1 == -INFINITY ? 0.0f : ex2(m1 - mm);
-            const float L = e0 * l + e1 * l1;
+        {
+            const float L = st[row].y + st[128 + row].y;
             const float inv = ns > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
+            const float back = mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f));
 #pragma unroll
-            for (int d = 0; d < HD; d++) so[d * 129 + row] = (e0 * acc[d] + e1 * so[d * 129 + row]) * inv;
-            st[4 * row + 2] = mm;
-            st[4 * row + 3] = L;
+            for (int d = 0; d < HC; d++) so[(half * HC + d) * 129 + row] = acc[d] * back * inv;
         }
         mn_group_sync();
         if (!*abortp) {
             // a warp per query, lanes over the head dim
-            for (int i = warp - 4; i < 128 && q0 + i < nq; i += 8) {
+            for (int i = warp - MN_LOADERS / 32; i < 128 && q0 + i < nq; i += 8) {
                 const int oq = q0 + i, orow = rq.row0 + oq / G, h = kvh * G + oq % G;
                 float *rec = a.part + (((size_t)orow * a.H + h) * a.S + split) * (HD + 4);
                 float *dst = ns > 1 ? rec + 4 : a.out + (size_t)orow * a.ldo + (size_t)h * HD;
 #pragma unroll
                 for (int d = lane; d < HD; d += 32) dst[d] = so[d * 129 + i];
-                if (ns > 1 && lane == 0) *reinterpret_cast<float2 *>(rec) = make_float2(st[4 * i + 2], st[4 * i + 3]);
+                if (ns > 1 && lane == 0)
+                    *reinterpret_cast<float2 *>(rec) = make_float2(st[i].x, st[i].y + st[128 + i].y);
             }
         }
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        if (warp == 12 && lane == 0) {
+        if (warp == 16 && lane == 0) {
             // ------------------------------ S = Q K^T ------------------------------
             const uint32_t idesc = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            bool go = nt > 0 && mn_wait(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);
 #pragma unroll 1
-            for (int j = 0; j < nt; j++) {
+            for (int j = 0; j < nt && go; j++) {
                 const int s = j & 1;
-                bool ok = mbar_wait(kfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+                bool ok = mn_wait(kfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
                 // the buffer's weights (tile j - 2) have been multiplied
-                if (ok && j >= 2) ok = mbar_wait(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                if (ok && j >= 2) ok = mn_wait(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t kb = smb + M::K + s * M::TILE, d = tmem + 128 * s;
@@ -414,19 +465,18 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     mma_f16_ts(d, t_q + 8 * k, bd, idesc, k != 0);
                     mma_f16_ts(d, t_q + 64 + 8 * k, bd, idesc, 1u);
                 }
-                mma_commit(kempty(s));
                 mma_commit(sfull(s));
             }
-        } else if (warp == 13 && lane == 0) {
+        } else if (warp == 17 && lane == 0) {
             // ------------------------------ O = P V ------------------------------
             // V is MN-major (bit 16): 8-column chunks MN_CHUNK apart, groups of 8 tokens 128 bytes apart
             const uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 #pragma unroll 1
             for (int j = 0; j < nt; j++) {
                 const int s = j & 1;
-                bool ok = mbar_wait(vfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
-                ok = ok && mbar_wait(pfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-                if (ok && j >= 1) ok = mbar_wait(oempty((j - 1) & 1), ((j - 1) >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                bool ok = mn_wait(vfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+                ok = ok && mn_wait(pfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                if (ok && j >= 1) ok = mn_wait(oempty, (j - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t vb = smb + M::V + s * M::TILE, p = tmem + 128 * s;
@@ -436,15 +486,14 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     mma_f16_ts(t_o, p + 16 * k, bd, idesc, k != 0);
                     mma_f16_ts(t_o, p + 16 * k + 8, bd, idesc, 1u);
                 }
-                mma_commit(vempty(s));
                 mma_commit(ofull(s));
             }
-        } else if (warp == 14 && lane < 8) {
+        } else if (warp == 18 && lane < 8) {
             // ------------------------------ blocks and scales ------------------------------
             const int *trow = a.table + (size_t)r * a.max_blocks;
             for (int j = 0; j < nt; j++) {
                 const int e = j % MN_PAGES;
-                if (j >= MN_PAGES && !mbar_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI)) break;
+                if (j >= MN_PAGES && !mn_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI)) break;
                 const int p = p0 + 128 * j + 16 * lane;
                 long long at = -1;
                 float ks = 0.0f, vs = 0.0f;
@@ -468,13 +517,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         }
         __syncwarp();
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     }
 
     // ------------------------------ end ------------------------------
-    if ((warp == 12 || warp == 13) && lane == 0 && *abortp) {
+    if ((warp == 16 || warp == 17) && lane == 0 && *abortp) {
         // an aborted issuer's products may still run: wait for them (bounded)
-        const uint32_t bar = bar0 + 8u * (warp == 12 ? 16 : 17);
+        const uint32_t bar = bar0 + 8u * (warp == 16 ? 16 : 17);
         mma_commit(bar);
         const uint64_t t1 = vxc_globaltimer();
         while (!mbar_try(bar, 0) && vxc_globaltimer() - t1 < 100000000ull) {}
@@ -483,7 +532,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) tmem_dealloc(tmem, 512u);
+    if (warp == 16) tmem_dealloc(tmem, 512u);
 }
 
 template <int TYPE>
