@@ -281,138 +281,217 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// A run = the rows of one block (they stand together in the slot map); CTA =
-// (window of rows, head, K or V) and goes over the runs that begin in its
-// window.  Two passes over a run's elements: their largest magnitude, then the
-// codes; the first AP_HELD float4 of each thread stay in registers in between
-// (a block of 64 tokens x 128 elements whole), the rest is read again from L2.
+// A run = the rows of one block (they stand together in the slot map).  CTA =
+// (window of rows, head, K or V), cut into teams of TS threads; each team goes
+// over runs that begin in the window.  Two passes over a run's elements: their
+// largest magnitude, then the codes; the first AP_HELD passes stay in registers
+// in between, the rest is read again from L2.  TS is chosen so that a block's
+// rows are AP_HELD passes, and the window so that a team has about one run: a
+// CTA that finds no run costs a slot on its SM for the time of a load (with
+// windows of 16 rows and blocks of 64 these took longer than the work).
 // Bytes bound it: 4 read and 1 written per element.
 #define AP_THREADS 256
 #define AP_HELD 8
 
-template <int TYPE, int HD>
-__global__ void __launch_bounds__(AP_THREADS)
+template <int TS>
+__device__ __forceinline__ void team_sync(int team) {
+    if (TS == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(TS) : "memory");
+}
+
+template <int TYPE, int TS>
+__global__ void __launch_bounds__(AP_THREADS, 4)
     k_kv8_append(const vxc_kv8 kv, const float *__restrict__ kx, long long ldk, const float *__restrict__ vx,
-                 long long ldv, const int *__restrict__ slot, int n_rows, int window, unsigned int *err) {
-    constexpr int C4 = HD / 4;   // float4 per row
-    __shared__ int win[KV8_MAX_BS];
+                 long long ldv, const int *__restrict__ slot, int n_rows, int window, int lsh, int units, unsigned int *err) {
+    constexpr int TEAMS = AP_THREADS / TS;
+    extern __shared__ int sm[];
     __shared__ float red[AP_THREADS / 32];
-    const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-    const int bs = kv.block_size, h = blockIdx.y, cap = kv.n_blocks * bs;
-    const float *x = (blockIdx.z ? vx : kx) + (size_t)h * HD;
-    const long long ld = blockIdx.z ? ldv : ldk;
-    uint8_t *codes = (uint8_t *)(blockIdx.z ? kv.v : kv.k);
-    float *scales = blockIdx.z ? kv.v_scale : kv.k_scale;
+    __shared__ int n_lead;
+    const int tid = threadIdx.x, lane = tid & 31, team = tid / TS, tt = tid % TS;
+    const int bs = kv.block_size, hd = kv.head_dim, cap = kv.n_blocks * bs;
+    // this CTA's parts of a row: K and V of head 0, K and V of head 1, ...
+    const int parts = (2 * kv.n_kv_heads + units - 1) / units, u0 = (int)(blockIdx.x % (unsigned)parts) * units;
+    const int u1 = min(u0 + units, 2 * kv.n_kv_heads);
+    const int len = window + bs + 33;   // the row before the window, a run that begins with its last row, a warp's look behind it
+    int *s_blk = sm, *s_off = s_blk + len, *lead = s_off + len, *win = lead + window + team * bs;
     pdl_trigger();
     pdl_wait();
-    // rows of the window that begin a run
-    const int i0 = blockIdx.x * window;
-    unsigned leaders;
-    {
-        const int i = i0 + lane;
-        bool lead = false;
-        if (lane < window && i < n_rows) {
-            const int s = slot[i], p = i ? slot[i - 1] : -1;
-            if (s >= 0 && s < cap) lead = p < 0 || p / bs != s / bs;
-            else if (s != -1 && h == 0 && w == 0) vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
-        }
-        leaders = __ballot_sync(0xffffffffu, lead);
+    // blocks and offsets of the row before the window, its rows, and as many as a run may go on
+    const int i0 = (int)(blockIdx.x / (unsigned)parts) * window;
+    if (tid == 0) n_lead = 0;
+    auto split = [&](int i, int &blk, int &off) {
+        const int s = i >= 0 && i < n_rows ? slot[i] : -1;
+        const bool ok = s >= 0 && s < cap;
+        blk = ok ? s / bs : -1;
+        off = ok ? s - blk * bs : 0;
+        return s;
+    };
+    for (int t = tid; t < len; t += AP_THREADS) {
+        const int s = split(i0 - 1 + t, s_blk[t], s_off[t]);
+        if (s != -1 && s_blk[t] < 0 && u0 == 0 && t >= 1 && t <= window) vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
     }
+    __syncthreads();
+    for (int t = tid; t < window; t += AP_THREADS)
+        if (s_blk[t + 1] >= 0 && s_blk[t + 1] != s_blk[t]) lead[atomicAdd(&n_lead, 1)] = t;   // (runs in any order)
+    __syncthreads();
+    const int c = tt & ((1 << lsh) - 1), jr = tt >> lsh, rpp = TS >> lsh;   // float4 of a row, row of a pass, rows a pass
+    const bool on = 4 * c < hd;
     bool odd = false;   // a NaN or infinity was stored as 0
-    while (leaders) {
-        const int first = i0 + __ffs(leaders) - 1;
-        leaders &= leaders - 1;
-        const int blk = slot[first] / bs;
+    for (int k = team; k < n_lead; k += TEAMS) {
+        const int t0 = lead[k] + 1, first = i0 + lead[k], blk = s_blk[t0];
+        // a run goes on past the table only if it has slots twice
+        auto blk_of = [&](int j) {
+            if (t0 + j < len) return s_blk[t0 + j];
+            int b, o;
+            split(first + j, b, o);
+            return b;
+        };
+        auto off_of = [&](int j) {
+            if (t0 + j < len) return s_off[t0 + j];
+            int b, o;
+            split(first + j, b, o);
+            return o;
+        };
+        // rows of the run; plain: their offsets ascend one by one, as from vxc_kv8_tables (then win is not needed)
+        const int off0 = s_off[t0];
         int n = 0;
+        bool plain = true;
+#pragma unroll 1
         for (bool more = true; more;) {
-            const int i = first + n + lane;
-            const int s = i < n_rows ? slot[i] : -1;
-            const unsigned in = __ballot_sync(0xffffffffu, s >= 0 && s / bs == blk);
+            const bool mine = blk_of(n + lane) == blk;
+            const unsigned in = __ballot_sync(0xffffffffu, mine);
+            const unsigned up = __ballot_sync(0xffffffffu, off_of(n + lane) == off0 + n + lane);
             more = in == 0xffffffffu;
-            n += more ? 32 : __ffs(~in) - 1;
+            const int k = more ? 32 : __ffs(~in) - 1;
+            plain = plain && (~up & (more ? 0xffffffffu : (1u << k) - 1u)) == 0;
+            n += k;
         }
-        __syncthreads();   // the last run's win and red are no longer read
-        for (int t = tid; t < bs; t += AP_THREADS) win[t] = -1;
-        __syncthreads();
-        for (int j = tid; j < n; j += AP_THREADS) atomicMax(&win[slot[first + j] % bs], j);
-        const int nu = n * C4;
-        auto load = [&](int u) {
-            float4 f = *reinterpret_cast<const float4 *>(x + (size_t)(first + u / C4) * ld + (size_t)(u % C4) * 4);
+        if (!plain) {
+            team_sync<TS>(team);   // the last run's win is no longer read
+            for (int t = tt; t < bs; t += TS) win[t] = -1;
+            team_sync<TS>(team);
+#pragma unroll 1
+            for (int j = tt; j < n; j += TS) atomicMax(&win[off_of(j)], j);
+            team_sync<TS>(team);
+        }
+        auto written = [&](int t) { return plain ? t >= off0 && t < off0 + n : win[t] >= 0; };
+        // NaN and infinity count as 0
+        auto finite = [](float4 f) {
             const float big = 3.402823466e38f;
-            if (!(fabsf(f.x) <= big)) { f.x = 0.0f; odd = true; }
-            if (!(fabsf(f.y) <= big)) { f.y = 0.0f; odd = true; }
-            if (!(fabsf(f.z) <= big)) { f.z = 0.0f; odd = true; }
-            if (!(fabsf(f.w) <= big)) { f.w = 0.0f; odd = true; }
+            f.x = fabsf(f.x) <= big ? f.x : 0.0f;
+            f.y = fabsf(f.y) <= big ? f.y : 0.0f;
+            f.z = fabsf(f.z) <= big ? f.z : 0.0f;
+            f.w = fabsf(f.w) <= big ? f.w : 0.0f;
             return f;
         };
         auto max4 = [](float4 f) { return fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))); };
-        float4 keep[AP_HELD];
-        float mx = 0.0f;
+        // 0, or NaN if one of the four is none or infinite
+        auto nan4 = [](float4 f, float t) { return fmaf(f.x, 0.0f, fmaf(f.y, 0.0f, fmaf(f.z, 0.0f, fmaf(f.w, 0.0f, t)))); };
+#pragma unroll 1
+        for (int u = u0; u < u1; u++) {
+            const int h = u >> 1, isv = u & 1;
+            const size_t ld4 = (size_t)(isv ? ldv : ldk) / 4;
+            const float4 *row = reinterpret_cast<const float4 *>((isv ? vx : kx) + (size_t)h * hd) + (size_t)first * ld4 + c;
+            auto load = [&](int j) { return row[(size_t)j * ld4]; };
+            float *sc = (isv ? kv.v_scale : kv.k_scale) + (size_t)blk * kv.n_kv_heads + h;
+            const float held = *sc;
+            float4 keep[AP_HELD];
+            {
+                const float4 *p = row + (size_t)jr * ld4;
+                const size_t step = (size_t)rpp * ld4;
 #pragma unroll
-        for (int i = 0; i < AP_HELD; i++) {
-            const int u = tid + i * AP_THREADS;
-            if (u < nu) {
-                keep[i] = load(u);
-                mx = fmaxf(mx, max4(keep[i]));
+                for (int i = 0; i < AP_HELD; i++) {
+                    keep[i] = on && jr + i * rpp < n ? *p : make_float4(0.f, 0.f, 0.f, 0.f);
+                    p += step;
+                }
             }
-        }
-        for (int u = tid + AP_HELD * AP_THREADS; u < nu; u += AP_THREADS) mx = fmaxf(mx, max4(load(u)));
-        mx = warp_max(mx);
-        if (lane == 0) red[w] = mx;
-        float *sc = scales + (size_t)blk * kv.n_kv_heads + h;
-        const float held = *sc;
-        __syncthreads();
-        mx = red[0];
+            team_sync<TS>(team);   // the last part's red is no longer read
+            float mx = 0.0f, nan = 0.0f;
 #pragma unroll
-        for (int i = 1; i < AP_THREADS / 32; i++) mx = fmaxf(mx, red[i]);
-        const float old = win[0] >= 0 ? 0.0f : held;
-        const float s = fmaxf(old, mx > 0.0f ? __uint_as_float((uint32_t)(kv8_scale_exp(mx, TYPE) + 127) << 23) : 0.0f);
-        uint8_t *dst = codes + ((size_t)blk * kv.n_kv_heads + h) * bs * HD;
-        if (s > old && old > 0.0f) {
-            // the scale grew: the tokens that stay are rounded again
-            const float ratio = old / s;
-            for (int u = tid; u < bs * HD / 4; u += AP_THREADS) {
-                if (win[u / C4] >= 0) continue;
-                uint32_t *p = reinterpret_cast<uint32_t *>(dst) + u;
-                const uint32_t q = *p;
-                *p = kv8_pack4<TYPE>(kv8_value<TYPE>(q & 0xFF) * ratio, kv8_value<TYPE>((q >> 8) & 0xFF) * ratio,
-                                     kv8_value<TYPE>((q >> 16) & 0xFF) * ratio, kv8_value<TYPE>(q >> 24) * ratio);
+            for (int i = 0; i < AP_HELD; i++) nan = nan4(keep[i], nan);
+#pragma unroll
+            for (int i = 0; i < AP_HELD; i++) mx = fmaxf(mx, max4(keep[i]));
+            // a thread with a NaN or an infinity reads its rows again, one by one
+            const bool bad = nan != 0.0f;
+            if (bad) {
+                odd = true;
+                mx = 0.0f;
             }
-        }
-        // dividing by a power of two is a product with its inverse; a scale that
-        // is none (written by the caller) is divided by
-        const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
-        const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-        auto store = [&](int u, float4 f) {
-            const int j = u / C4, off = slot[first + j] % bs;
-            if (win[off] != j) return;   // a later row has this slot
-            if (pow2 || s == 0.0f) {
-                f.x *= inv, f.y *= inv, f.z *= inv, f.w *= inv;
+#pragma unroll 1
+            for (int j = jr + (bad ? 0 : AP_HELD * rpp); on && j < n; j += rpp) {
+                const float4 f = load(j);
+                if (nan4(f, 0.0f) != 0.0f) odd = true;
+                mx = fmaxf(mx, max4(finite(f)));
+            }
+            mx = warp_max(mx);
+            if (TS > 32) {
+                if (lane == 0) red[tid >> 5] = mx;
+                team_sync<TS>(team);
+#pragma unroll
+                for (int i = 0; i < TS / 32; i++) mx = fmaxf(mx, red[team * (TS / 32) + i]);
             } else {
-                f.x /= s, f.y /= s, f.z /= s, f.w /= s;
+                __syncwarp();
             }
-            *reinterpret_cast<uint32_t *>(dst + (size_t)off * HD + (size_t)(u % C4) * 4) = kv8_pack4<TYPE>(f.x, f.y, f.z, f.w);
-        };
+            const float old = written(0) ? 0.0f : held;
+            const float s = fmaxf(old, mx > 0.0f ? __uint_as_float((uint32_t)(kv8_scale_exp(mx, TYPE) + 127) << 23) : 0.0f);
+            uint8_t *dst = (uint8_t *)(isv ? kv.v : kv.k) + ((size_t)blk * kv.n_kv_heads + h) * bs * hd;
+            if (s > old && old > 0.0f) {
+                // the scale grew: the tokens that stay are rounded again
+                const float ratio = old / s;
+#pragma unroll 1
+                for (int j = jr; on && j < bs; j += rpp) {
+                    if (written(j)) continue;
+                    uint32_t *p = reinterpret_cast<uint32_t *>(dst + (size_t)j * hd) + c;
+                    const uint32_t q = *p;
+                    *p = kv8_pack4<TYPE>(kv8_value<TYPE>(q & 0xFF) * ratio, kv8_value<TYPE>((q >> 8) & 0xFF) * ratio,
+                                         kv8_value<TYPE>((q >> 16) & 0xFF) * ratio, kv8_value<TYPE>(q >> 24) * ratio);
+                }
+            }
+            // dividing by a power of two is a product with its inverse; a scale that
+            // is none (written by the caller) is divided by
+            const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
+            const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+            auto store = [&](int off, float4 f) {
+                uint32_t *to = reinterpret_cast<uint32_t *>(dst + (size_t)off * hd) + c;
+                if (pow2 || s == 0.0f)
+                    *to = TYPE == VXC_KV8_INT8 ? kv8_pack4_int8(f.x, f.y, f.z, f.w, inv)
+                                               : kv8_pack4<TYPE>(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+                else
+                    *to = kv8_pack4<TYPE>(f.x / s, f.y / s, f.z / s, f.w / s);
+            };
+            int held_rows = 0;   // rows stored from registers
+            if (plain && pow2 && !bad) {
+                uint32_t *to = reinterpret_cast<uint32_t *>(dst + (off0 + jr) * hd) + c;
+                const int step = rpp * hd / 4;
 #pragma unroll
-        for (int i = 0; i < AP_HELD; i++) {
-            const int u = tid + i * AP_THREADS;
-            if (u < nu) store(u, keep[i]);
+                for (int i = 0; i < AP_HELD; i++) {
+                    if (on && jr + i * rpp < n)
+                        to[i * step] =
+                            TYPE == VXC_KV8_INT8 ? kv8_pack4_int8(keep[i].x, keep[i].y, keep[i].z, keep[i].w, inv)
+                                                 : kv8_pack4<TYPE>(keep[i].x * inv, keep[i].y * inv, keep[i].z * inv, keep[i].w * inv);
+                }
+                held_rows = AP_HELD * rpp;
+            }
+#pragma unroll 1
+            for (int j = jr + held_rows; on && j < n; j += rpp) {
+                const int off = off_of(j);
+                if (plain || win[off] == j) store(off, finite(load(j)));   // (not if a later row has this slot)
+            }
+            if (tt == 0 && s != held) *sc = s;
         }
-        for (int u = tid + AP_HELD * AP_THREADS; u < nu; u += AP_THREADS) store(u, load(u));
-        if (tid == 0 && s != held) *sc = s;
     }
     if (__any_sync(0xffffffffu, odd) && lane == 0) vxc_flag_error(err, VXC_DERR_NONFINITE);
 }
 
 typedef void (*append_kernel_t)(const vxc_kv8, const float *, long long, const float *, long long, const int *, int,
-                                int, unsigned int *);
+                                int, int, int, unsigned int *);
 template <int TYPE>
-static append_kernel_t append_kernel(int hd) {
-    switch (hd) {
+static append_kernel_t append_kernel(int ts) {
+    switch (ts) {
         case 32: return k_kv8_append<TYPE, 32>;
         case 64: return k_kv8_append<TYPE, 64>;
-        case 96: return k_kv8_append<TYPE, 96>;
-        default: return k_kv8_append<TYPE, 128>;
+        case 128: return k_kv8_append<TYPE, 128>;
+        default: return k_kv8_append<TYPE, 256>;
     }
 }
 
@@ -431,13 +510,26 @@ extern "C" int vxc_kv8_append(const vxc_kv8 *kv, const float *k, long long ldk, 
     }
     if (int rc = vxc_require_device()) return rc;
     if (n_rows == 0) return 0;
-    // One row per CTA while all CTAs then fit the GPU at once or nearly so (a
-    // decode or verify step); else 16, the shortest run of whole blocks.
-    const int window = n_rows <= 512 ? 1 : 16;
-    append_kernel_t f = kv->type == VXC_KV8_INT8 ? append_kernel<VXC_KV8_INT8>(kv->head_dim)
-                                                 : append_kernel<VXC_KV8_E4M3>(kv->head_dim);
-    VXC_CUDA_OK(kv8_launch(f, dim3((n_rows + window - 1) / window, kv->n_kv_heads, 2), dim3(AP_THREADS), 0,
-                           (cudaStream_t)stream, 1, *kv, k, ldk, v, ldv, d_slot, n_rows, window,
+    const int bs = kv->block_size, lsh = kv->head_dim == 32 ? 3 : kv->head_dim == 64 ? 4 : 5;
+    // threads for a block's rows in AP_HELD passes
+    int ts = 32;
+    while (ts < AP_THREADS && (ts >> lsh) * AP_HELD < bs) ts *= 2;
+    // rows per CTA: as many as keep two rounds of CTAs on the GPU (4 fit an SM), at most a block per
+    // team: a step's few rows, each probably in a block of its own, go to as many CTAs
+    const int most = AP_THREADS / ts * bs;
+    const long long even = ((long long)n_rows * kv->n_kv_heads * 2 + 2 * 4 * 148 - 1) / (2 * 4 * 148);
+    const int window = even < 1 ? 1 : even < most ? (int)even : most;
+    // K and V of two heads per CTA when there are CTAs enough: a run is looked up once for them
+    const int units = even >= 4ll * most ? 4 : 1;
+    const size_t smem = (size_t)(2 * (window + bs + 33) + window + AP_THREADS / ts * bs) * sizeof(int);
+    append_kernel_t f = kv->type == VXC_KV8_INT8 ? append_kernel<VXC_KV8_INT8>(ts) : append_kernel<VXC_KV8_E4M3>(ts);
+    const long long grid = (long long)((n_rows + window - 1) / window) * ((2 * kv->n_kv_heads + units - 1) / units);
+    if (grid > INT_MAX) {
+        vxc_set_error("vxc_kv8_append: %d rows of %d heads", n_rows, kv->n_kv_heads);
+        return -4;
+    }
+    VXC_CUDA_OK(kv8_launch(f, dim3((unsigned)grid), dim3(AP_THREADS), smem,
+                           (cudaStream_t)stream, 1, *kv, k, ldk, v, ldv, d_slot, n_rows, window, lsh, units,
                            vxc_device_error_ptr()));
     return 0;
 }

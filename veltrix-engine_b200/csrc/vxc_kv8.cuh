@@ -22,15 +22,21 @@ __device__ __forceinline__ int kv8_scale_exp(float amax, int type) {
     return e < -126 ? -126 : e;
 }
 
+// Four integer codes of x * inv, inv a power of two, |x * inv| <= 127: the sum
+// with 1.5 * 2^23 is rounded to an integer (once: the product is exact), which
+// its low byte holds.
+__device__ __forceinline__ uint32_t kv8_pack4_int8(float a, float b, float c, float d, float inv) {
+    const float big = 12582912.0f;
+    const uint32_t x = __float_as_uint(__fmaf_rn(a, inv, big)), y = __float_as_uint(__fmaf_rn(b, inv, big));
+    const uint32_t z = __float_as_uint(__fmaf_rn(c, inv, big)), w = __float_as_uint(__fmaf_rn(d, inv, big));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
 // Four codes of x[] (already in units of the scale) as one word, to nearest,
 // ties to even.
 template <int TYPE>
 __device__ __forceinline__ uint32_t kv8_pack4(float a, float b, float c, float d) {
-    if (TYPE == VXC_KV8_INT8) {
-        const uint32_t lo = ((uint32_t)__float2int_rn(a) & 0xFFu) | (((uint32_t)__float2int_rn(b) & 0xFFu) << 8);
-        const uint32_t hi = ((uint32_t)__float2int_rn(c) & 0xFFu) | (((uint32_t)__float2int_rn(d) & 0xFFu) << 8);
-        return lo | (hi << 16);
-    }
+    if (TYPE == VXC_KV8_INT8) return kv8_pack4_int8(a, b, c, d, 1.0f);
     uint16_t lo, hi;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
