@@ -10,8 +10,9 @@
 // CTA = (request, kv head, chunk of NQ queries) x one split of the request's
 // tokens.  Queries are the request's rows times the heads of the kv head,
 // query = row * G + head, so every byte of the split is read once for all.
-// Each of the 4 warps goes over every fourth tile of 16 tokens, with a softmax
-// state and an output of its own; the warps are joined at the end.
+// Each of the 4 warps goes over every fourth piece of 32 tokens (two tiles of
+// 16), with a softmax state and an output of its own; the warps are joined at
+// the end.
 //
 // Products.  mma m16n8k16 in fp16 with fp32 sums.  A code is exact in fp16.  A
 // query row is scaled by a power of two and split into two fp16 parts, hi and
@@ -20,13 +21,17 @@
 //     their two sums are added: one instruction does both products.
 //   NQ = 16: two instructions into the same sums, hi and lo.
 // Layouts.  The sum over the head dim may go in any order, so lane t of a quad
-// takes the pieces of a K row that it can load as whole words (Kv8Piece::k_at), and
-// the query's fragment is loaded in the same order.  Likewise the output's
-// columns: lane group g takes pieces of a V row (Kv8Piece::v_at).  So every byte goes
-// by cp.async to the ring slot of the lane that uses it, and back from there
-// without a bank conflict; no lane reads another's bytes and the ring needs no
-// barrier.  Scores come out where the weights' fragment wants them: lane (g, t)
-// has tokens 2t, 2t+1, 2t+8, 2t+9 of query g, and loads V of just these.
+// takes the pieces of a K row that it can load as whole words (Kv8Few::k_at),
+// and the query's fragment is loaded in the same order.  Likewise the output's
+// columns: lane group g takes pieces of a V row (Kv8Few::v_at).  Scores come out
+// where the weights' fragment wants them: lane (g, t) has tokens 2t, 2t+1,
+// 2t+8, 2t+9 of query g, and reads V of just these.
+// A tile (16 rows) is one contiguous span of its block; it comes by cp.async,
+// 512 bytes an instruction, to the warp's own ring, its 16-byte chunks exchanged
+// within 128 bytes so that both reads are free of bank conflicts at head dims 64
+// and 128.  (With every lane fetching the bytes it uses itself an instruction
+// touched 8 lines for K and 16 for V instead of 4, and issuing took a third of
+// the time.)
 // Softmax in base 2 with two running maxima per query: m of the scores s, for
 // the sum l of 2^(s - m), and mv of s + log2(v_scale), the reference of the
 // weights w = 2^(s - mv) v_scale 2^KV8_HEAD that multiply the codes of V: a
@@ -35,21 +40,30 @@
 // seldom rescaled.
 // Tokens behind the request's last one and blocks outside the cache are read
 // as zeros (cp.async's zero fill), so nothing of theirs reaches a product.
+// The blocks and scales of the split are looked up once, at the start.
 // ---------------------------------------------------------------------------
-#define FEW_STAGES 4     // 16-token tiles in flight per warp
+#define FEW_STAGES 3     // 32-token pieces per warp: one in use, the others in flight
 
-// Bytes that one cp.async brings, and the offset of piece c in a row.
 template <int HD>
-struct Kv8Piece {
-    static constexpr int K = HD % 64 == 0 ? 16 : 8, NK = HD / 4 / K;                    // of a K row, lane t of a quad
-    static constexpr int V = HD == 128 ? 16 : HD == 64 ? 8 : 4, NV = HD / 8 / V;        // of a V row, lane group g
+struct Kv8Few {
+    // pieces (bytes, count, place in the row) of a K row that lane t of a quad reads, of a V row that lane group g reads
+    static constexpr int K = HD % 64 == 0 ? 16 : 8, NK = HD / 4 / K;
+    static constexpr int V = HD == 128 ? 16 : HD == 64 ? 8 : 4, NV = HD / 8 / V;
     static __device__ __forceinline__ int k_at(int c, int t) { return c * 4 * K + t * K; }
     static __device__ __forceinline__ int v_at(int c, int g) { return c * 8 * V + g * V; }
+    // place of byte `at` of row `row` in a tile of the ring (at a multiple of the piece)
+    static __device__ __forceinline__ int k_slot(int row, int at) {
+        const int b = row * HD + at;
+        return HD == 128 ? b ^ ((row & 1) << 6) : b;
+    }
+    static __device__ __forceinline__ int v_slot(int row, int at) {
+        const int b = row * HD + at;
+        return HD == 128 ? b ^ ((row & 6) << 4) : HD == 64 ? b ^ ((row & 6) << 4) : b;
+    }
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -57,12 +71,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // Records of the splits: [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum
 // of 2^(s - m) v.
 template <int TYPE, int HD, int NQ>
-__global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8AttnArgs a) {
-    using P = Kv8Piece<HD>;
+__global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
+    using P = Kv8Few<HD>;
     constexpr int NR = NQ / 8;                 // query rows per lane
     constexpr int KS = HD / 16;                // steps over the head dim
     constexpr int NT = HD / 8;                 // column tiles of the output
-    constexpr int STAGE = HD * 32 + 16;        // a tile's codes, its two scales
+    constexpr int TILE = HD * 32;              // bytes of K and V of 16 tokens
+    constexpr int STAGE = 2 * TILE;
     extern __shared__ __align__(16) unsigned char sm[];
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
@@ -78,6 +93,24 @@ __global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8
     if (split >= ns) return;
     // visible tokens of the chunk's last query end this CTA's range
     const int p0 = split * SL, p1 = min(p0 + SL, rq.pos + (min(q0 + NQ, nq) - 1) / G + 1);
+
+    // blocks and scales of the split: {block (-1: outside the cache), K scale, V scale, its logarithm}
+    float4 *pages = reinterpret_cast<float4 *>(sm + 4 * FEW_STAGES * STAGE);
+    const int e0 = p0 / bs, ne = p1 > p0 ? (p1 - 1) / bs - e0 + 1 : 0;
+    for (int i = tid; i < ne; i += 128) {
+        const int b = a.table[(size_t)r * a.max_blocks + e0 + i];
+        float4 e = make_float4(__int_as_float(-1), 0.0f, 0.0f, -INFINITY);
+        if (b >= 0 && b < a.kv.n_blocks) {
+            const size_t bh = (size_t)b * KH + kvh;
+            e.x = __int_as_float(b);
+            e.y = a.kv.k_scale[bh];
+            e.z = a.kv.v_scale[bh];
+            e.w = lg2(e.z);
+        } else {
+            vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+        }
+        pages[i] = e;
+    }
 
     // queries: fragments hi (and lo), the factor of each row's scores
     uint32_t qf[NR == 1 ? 1 : 2][KS][4];
@@ -124,45 +157,45 @@ __global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8
 #pragma unroll
     for (int i = 0; i < NR; i++) m[i] = mv[i] = -INFINITY, l[i] = 0.0f;
 
-    // tiles w, w + 4, ... of the range
-    const int ntile = p1 > p0 ? (p1 - p0 + 15) >> 4 : 0, nit = ntile > w ? (ntile - w + 3) >> 2 : 0;
+    // pieces w, w + 4, ... of the range
+    const int npc = p1 > p0 ? (p1 - p0 + 31) >> 5 : 0, nit = npc > w ? (npc - w + 3) >> 2 : 0;
     unsigned char *ring = sm + w * (FEW_STAGES * STAGE);
     const uint32_t ring_u = smem_u32(ring);
-    const int *trow = a.table + (size_t)r * a.max_blocks;
     const int bs16 = bs >> 4;
-    int blk = (p0 / 16 + w) / bs16, off16 = (p0 / 16 + w) % bs16;   // of the next tile to issue
-    int p_issue = p0 + 16 * w;
-    int b_next = nit > 0 ? trow[blk] : -1;
-    uint32_t bad = 0;   // stages whose block is outside the cache
+    const uint8_t *kb = (const uint8_t *)a.kv.k + (size_t)kvh * bs * HD + lane * 16;
+    const uint8_t *vb = (const uint8_t *)a.kv.v + (size_t)kvh * bs * HD + lane * 16;
+    const size_t bstep = (size_t)KH * bs * HD;
+    const int tile0 = p0 / 16 - e0 * bs16 + 2 * w;   // the warp's first tile, counted from the first page's start
+    int pi = tile0 / bs16, oi = tile0 % bs16;        // page and tile in it of the next tile to bring in
+    int pc = pi, oc = oi;                            // and of the next one to use
+    int p_in = p0 + 32 * w;
+    __syncthreads();   // pages
     auto issue = [&](int it) {
         if (it < nit) {
-            const int st = it % FEW_STAGES;
-            const bool ok = b_next >= 0 && b_next < a.kv.n_blocks;
-            bad = (bad & ~(1u << st)) | (ok ? 0u : 1u << st);
-            const size_t bh = (size_t)(ok ? b_next : 0) * KH + kvh;
-            const size_t at = (bh * bs + (size_t)off16 * 16) * HD;
-            const uint8_t *ks = (const uint8_t *)a.kv.k + at, *vs = (const uint8_t *)a.kv.v + at;
-            const uint32_t base = ring_u + st * STAGE;
-            const int live = ok ? rq.kvlen - p_issue : 0;   // tokens of the tile that exist
+            uint32_t dst = ring_u + it % FEW_STAGES * STAGE;
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int u = 0; u < 2; u++) {
+                const int blk = p_in < p1 ? __float_as_int(pages[pi].x) : -1;
+                const size_t at = (size_t)max(blk, 0) * bstep + (size_t)(oi * 16) * HD;
+                const uint8_t *ks = kb + at, *vs = vb + at;
+                const int live = blk >= 0 ? rq.kvlen - p_in : 0;   // tokens of the tile that exist
+                // instruction k brings chunks 32 k + lane of the span
+                auto bring = [&](auto copy) {
 #pragma unroll
-                for (int c = 0; c < P::NK; c++)
-                    cp_async_zfill<P::K>(base + (n * P::NK + c) * 32 * P::K + lane * P::K,
-                                         ks + (n * 8 + g) * HD + P::k_at(c, t), n * 8 + g < live);
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const int tok = (n >> 1) * 8 + 2 * t + (n & 1);
-#pragma unroll
-                for (int c = 0; c < P::NV; c++)
-                    cp_async_zfill<P::V>(base + HD * 16 + (n * P::NV + c) * 32 * P::V + lane * P::V,
-                                         vs + tok * HD + P::v_at(c, g), tok < live);
+                    for (int k = 0; k < HD / 32; k++) {
+                        const int byte = k * 512 + lane * 16, row = byte / HD, in = byte % HD;
+                        copy(dst + P::k_slot(row, in), ks + k * 512, row);
+                        copy(dst + HD * 16 + P::v_slot(row, in), vs + k * 512, row);
+                    }
+                };
+                if (live >= 16) bring([](uint32_t d, const uint8_t *x, int) { cp_async<16>(d, x); });
+                else bring([&](uint32_t d, const uint8_t *x, int row) { cp_async_zfill<16>(d, x, row < live); });
+                dst += TILE;
+                p_in += 16;
+                oi += u == 0 ? 1 : 7;   // the pair's second tile; the warp's next piece
+                while (oi >= bs16) oi -= bs16, pi++;
             }
-            if (lane < 2) cp_async_zfill<4>(base + HD * 32 + 4 * lane, (lane ? a.kv.v_scale : a.kv.k_scale) + bh, ok);
-            p_issue += 64;
-            off16 += 4;
-            while (off16 >= bs16) off16 -= bs16, blk++;
-            if (it + 1 < nit) b_next = trow[blk];
+            p_in += 96;
         }
         cp_commit();
     };
@@ -172,67 +205,84 @@ __global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8
     }
 #pragma unroll 1
     for (int it = 0; it < nit; it++) {
-        __syncwarp();   // the stage's scales have been read by every lane
-        const uint32_t was_bad = bad;
+        __syncwarp();   // every lane has read the piece that is replaced
         issue(it + FEW_STAGES - 1);
         cp_wait<FEW_STAGES - 1>();
-        __syncwarp();
+        __syncwarp();   // every lane's copies have landed
         const unsigned char *stg = ring + (it % FEW_STAGES) * STAGE;
-        const float kscale = *reinterpret_cast<const float *>(stg + HD * 32);
-        const float vscale = *reinterpret_cast<const float *>(stg + HD * 32 + 4);
-        const bool is_bad = (was_bad >> (it % FEW_STAGES)) & 1u;
-        if (is_bad && lane == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+        const int p = p0 + 32 * (w + 4 * it) + 2 * t;   // lane's tokens p, p + 1, p + 8, p + 9 of each tile
         // scores
-        float sc[2][4];
+        float sc[2][2][4], ksc[2], vsc[2], lv[2];
+        bool none[2];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+        for (int u = 0; u < 2; u++) {
+            const float4 e = p0 + 32 * (w + 4 * it) + 16 * u < p1 ? pages[pc] : make_float4(__int_as_float(-1), 0.f, 0.f, -INFINITY);
+            none[u] = __float_as_int(e.x) < 0;
+            ksc[u] = e.y, vsc[u] = e.z, lv[u] = e.w;
+            oc += u == 0 ? 1 : 7;
+            while (oc >= bs16) oc -= bs16, pc++;
+#pragma unroll
+            for (int n = 0; n < 2; n++) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
 #pragma unroll
             for (int c = 0; c < P::NK; c++) {
-                uint32_t word[P::K / 4];
-                const unsigned char *src = stg + (n * P::NK + c) * 32 * P::K + lane * P::K;
-                if (P::K == 16) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(src);
-                    word[0] = x.x, word[1] = x.y, word[P::K / 4 - 2] = x.z, word[P::K / 4 - 1] = x.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                    word[0] = x.x, word[1] = x.y;
+                uint32_t word[2][P::K / 4];
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const unsigned char *src = stg + u * TILE + n * 8 * HD + P::k_slot(g, P::k_at(c, t));
+                    if (P::K == 16) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                        word[n][0] = x.x, word[n][1] = x.y, word[n][P::K / 4 - 2] = x.z, word[n][P::K / 4 - 1] = x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                        word[n][0] = x.x, word[n][1] = x.y;
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < P::K / 4; e++) {
                     const int s = c * (P::K / 4) + e;
-                    uint32_t b0, b1;
-                    codes_h2<TYPE>(word[e], b0, b1);
-                    mma16816(sc[n], qf[0][s], b0, b1);
-                    if (NR == 2) mma16816(sc[n], qf[NR - 1][s], b0, b1);
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        uint32_t b0, b1;
+                        codes_h2<TYPE>(word[n][e], b0, b1);
+                        mma16816(sc[u][n], qf[0][s], b0, b1);
+                        if (NR == 2) mma16816(sc[u][n], qf[NR - 1][s], b0, b1);
+                    }
                 }
             }
         }
-        // weights: lane's tokens p, p + 1, p + 8, p + 9
-        const int p = p0 + 16 * (w + 4 * it) + 2 * t;
-        const float lv = lg2(vscale);
-        uint32_t wf[NR == 1 ? 1 : 2][4];
+        // weights
+        uint32_t wf[2][NR == 1 ? 1 : 2][4];
 #pragma unroll
         for (int i = 0; i < NR; i++) {
-            const float fk = f[i] * kscale;
-            float s[4];
-            if (NR == 1) {
-                s[0] = sc[0][0] + sc[0][2], s[1] = sc[0][1] + sc[0][3];
-                s[2] = sc[1][0] + sc[1][2], s[3] = sc[1][1] + sc[1][3];
-            } else {
-                s[0] = sc[0][2 * i], s[1] = sc[0][2 * i + 1], s[2] = sc[1][2 * i], s[3] = sc[1][2 * i + 1];
-            }
-            const int end = is_bad ? -1 : lim[i];
+            float s[2][4], mx[2];
 #pragma unroll
-            for (int k = 0; k < 4; k++) s[k] = p + (k & 1) + (k >> 1) * 8 <= end ? s[k] * fk : -INFINITY;
-            float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (mx > m[i] + KV8_LAG || (m[i] == -INFINITY && mx > m[i])) {
-                l[i] *= ex2(m[i] - mx);   // 0 at first
-                m[i] = mx;
+            for (int u = 0; u < 2; u++) {
+                const float fk = f[i] * ksc[u];
+                const float (&x)[2][4] = sc[u];
+                if (NR == 1) {
+                    s[u][0] = x[0][0] + x[0][2], s[u][1] = x[0][1] + x[0][3];
+                    s[u][2] = x[1][0] + x[1][2], s[u][3] = x[1][1] + x[1][3];
+                } else {
+                    s[u][0] = x[0][2 * i], s[u][1] = x[0][2 * i + 1], s[u][2] = x[1][2 * i], s[u][3] = x[1][2 * i + 1];
+                }
+                const int end = none[u] ? -1 : lim[i];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    s[u][k] = p + 16 * u + (k & 1) + (k >> 1) * 8 <= end ? s[u][k] * fk : -INFINITY;
+                mx[u] = fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3]));
             }
-            const float mxv = mx + lv;
+            float mm = fmaxf(mx[0], mx[1]), mxv = fmaxf(mx[0] + lv[0], mx[1] + lv[1]);
+            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, 1));
+            mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 1));
+            mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, 2));
+            mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 2));
+            if (mm > m[i] + KV8_LAG || (m[i] == -INFINITY && mm > m[i])) {
+                l[i] *= ex2(m[i] - mm);   // 0 at first
+                m[i] = mm;
+            }
             float shrink = 1.0f;
             if (mxv > mv[i] + KV8_LAG || (mv[i] == -INFINITY && mxv > mv[i])) {
                 shrink = ex2(mv[i] - mxv);
@@ -249,53 +299,60 @@ __global__ void __launch_bounds__(128, NQ == 8 ? 3 : 2) k_kv8_attn_few(const Kv8
                 }
             }
             const float mref = m[i] == -INFINITY ? 0.0f : m[i];
-            const float c = vscale * ex2(fminf(mref - mv[i] + KV8_HEAD, 120.0f));
+            const float cv = ex2(fminf(mref - mv[i] + KV8_HEAD, 120.0f));
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                s[k] = ex2(s[k] - mref);
-                l[i] += s[k];
-                s[k] *= c;
-            }
-            uint32_t l0, l1;
-            const uint32_t h0 = split_h2(s[0], s[1], l0), h1 = split_h2(s[2], s[3], l1);
-            if (NR == 1) {
-                wf[0][0] = h0, wf[0][1] = l0, wf[0][2] = h1, wf[0][3] = l1;
-            } else {
-                wf[0][i] = h0, wf[0][2 + i] = h1;
-                wf[NR - 1][i] = l0, wf[NR - 1][2 + i] = l1;
+            for (int u = 0; u < 2; u++) {
+                const float c = vsc[u] * cv;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    s[u][k] = ex2(s[u][k] - mref);
+                    l[i] += s[u][k];
+                    s[u][k] *= c;
+                }
+                uint32_t l0, l1;
+                const uint32_t h0 = split_h2(s[u][0], s[u][1], l0), h1 = split_h2(s[u][2], s[u][3], l1);
+                if (NR == 1) {
+                    wf[u][0][0] = h0, wf[u][0][1] = l0, wf[u][0][2] = h1, wf[u][0][3] = l1;
+                } else {
+                    wf[u][0][i] = h0, wf[u][0][2 + i] = h1;
+                    wf[u][NR - 1][i] = l0, wf[u][NR - 1][2 + i] = l1;
+                }
             }
         }
         // weights times V: byte j of the lane's piece of tokens 2t, 2t+1, 2t+8, 2t+9 is column tile j
-        const unsigned char *vst = stg + HD * 16 + lane * P::V;
 #pragma unroll
-        for (int c = 0; c < P::NV; c++) {
-            uint32_t tok[4][P::V / 4];
+        for (int u = 0; u < 2; u++) {
+            const unsigned char *vst = stg + u * TILE + HD * 16;
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const unsigned char *src = vst + (n * P::NV + c) * 32 * P::V;
-                if (P::V == 16) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(src);
-                    tok[n][0] = x.x, tok[n][P::V / 4 > 1 ? 1 : 0] = x.y;
-                    tok[n][P::V / 4 > 2 ? 2 : 0] = x.z, tok[n][P::V / 4 - 1] = x.w;
-                } else if (P::V == 8) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                    tok[n][0] = x.x, tok[n][P::V / 4 - 1] = x.y;
-                } else {
-                    tok[n][0] = *reinterpret_cast<const uint32_t *>(src);
+            for (int c = 0; c < P::NV; c++) {
+                uint32_t tok[4][P::V / 4];
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const unsigned char *src = vst + (n >> 1) * 8 * HD + P::v_slot(2 * t + (n & 1), P::v_at(c, g));
+                    if (P::V == 16) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                        tok[n][0] = x.x, tok[n][P::V / 4 > 1 ? 1 : 0] = x.y;
+                        tok[n][P::V / 4 > 2 ? 2 : 0] = x.z, tok[n][P::V / 4 - 1] = x.w;
+                    } else if (P::V == 8) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                        tok[n][0] = x.x, tok[n][P::V / 4 - 1] = x.y;
+                    } else {
+                        tok[n][0] = *reinterpret_cast<const uint32_t *>(src);
+                    }
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < P::V / 4; e++) {
-                uint32_t b0[4], b1[4];
-                codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x5140), b0[0], b0[1]);
-                codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x7362), b0[2], b0[3]);
-                codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x5140), b1[0], b1[1]);
-                codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x7362), b1[2], b1[3]);
+                for (int e = 0; e < P::V / 4; e++) {
+                    uint32_t b0[4], b1[4];
+                    codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x5140), b0[0], b0[1]);
+                    codes_h2<TYPE>(__byte_perm(tok[0][e], tok[1][e], 0x7362), b0[2], b0[3]);
+                    codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x5140), b1[0], b1[1]);
+                    codes_h2<TYPE>(__byte_perm(tok[2][e], tok[3][e], 0x7362), b1[2], b1[3]);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int j = c * P::V + 4 * e + k;
-                    mma16816(o[j], wf[0], b0[k], b1[k]);
-                    if (NR == 2) mma16816(o[j], wf[NR - 1], b0[k], b1[k]);
+                    for (int k = 0; k < 4; k++) {
+                        const int j = c * P::V + 4 * e + k;
+                        mma16816(o[j], wf[u][0], b0[k], b1[k]);
+                        if (NR == 2) mma16816(o[j], wf[u][NR - 1], b0[k], b1[k]);
+                    }
                 }
             }
         }
@@ -416,6 +473,7 @@ struct AttnPlan {
     int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), KV8_TILE_Q (k_kv8_attn_many)
     int chunks;    // chunks per (request, kv head) at most, or tiles of all requests
     int S, sl_min;
+    int sl_max;    // tokens of a split at most
 };
 #ifndef ATTN_FEW_MAX
 #define ATTN_FEW_MAX 16   // queries of a request and kv head up to which k_kv8_attn_few is used
@@ -450,6 +508,8 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
     // warp, 5e-6 at most
     if (p.nq < KV8_TILE_Q && S < (tokens + 8191) / 8192) S = (tokens + 8191) / 8192;
     p.S = (int)(S < 1 ? 1 : S);
+    const long long even = (tokens + p.S - 1) / p.S;
+    p.sl_max = (int)(((even > p.sl_min ? even : p.sl_min) + 127) & ~127ll);
     return p;
 }
 
@@ -512,7 +572,7 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
         VXC_CUDA_OK(kv8_attn_many(a, p.chunks, (cudaStream_t)stream));
     } else {
         attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
-        size_t smem = (size_t)4 * FEW_STAGES * (hd * 32 + 16);
+        size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)(p.sl_max / kv->block_size + 2) * sizeof(float4);
         const size_t join = (size_t)4 * p.nq * (hd + 6) * sizeof(float);
         if (smem < join) smem = join;
         VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
