@@ -3,12 +3,15 @@
 //   out_i,h = sum_j softmax_j(scale q_i,h . k_j) v_j,  j <= position of row i
 #include "vxc_kv8_attn.cuh"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 // ---------------------------------------------------------------------------
 // Few queries per kv head (decode and small verify steps): split over the
 // context, warp-level tensor instructions.
 //
-// CTA = (request, kv head, chunk of NQ queries) x one split of the request's
-// tokens.  Queries are the request's rows times the heads of the kv head,
+// CTA = (request, kv head) x one split of the request's tokens.  Queries are the request's rows times the heads of the kv head,
 // query = row * G + head, so every byte of the split is read once for all.
 // Each of the 4 warps goes over every fourth piece of 32 tokens (two tiles of
 // 16), with a softmax state and an output of its own; the warps are joined at
@@ -42,7 +45,7 @@
 // as zeros (cp.async's zero fill), so nothing of theirs reaches a product.
 // The blocks and scales of the split are looked up once, at the start.
 // ---------------------------------------------------------------------------
-#define FEW_STAGES 3     // 32-token pieces per warp: one in use, the others in flight
+#define FEW_STAGES 2     // 32-token pieces per warp: one in use, one in flight (3: no faster, 4: fewer CTAs per SM, slower)
 
 template <int HD>
 struct Kv8Few {
@@ -68,8 +71,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Records of the splits: [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum
-// of 2^(s - m) v.
+// The splits of a request and head are joined by their cluster, through
+// distributed shared memory, while a cluster holds them all (a.S <= 8); else
+// they leave records in device memory for k_kv8_attn_join:
+// [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum of 2^(s - m) v.
 template <int TYPE, int HD, int NQ>
 __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     using P = Kv8Few<HD>;
@@ -83,33 +88,86 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
     pdl_trigger();
     pdl_wait();
-    const int r = blockIdx.z, kvh = blockIdx.x % KH, q0 = (blockIdx.x / KH) * NQ, split = blockIdx.y;
+    const int r = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
     const Kv8Req rq = kv8_req(a, r);
-    if (rq.over && blockIdx.x == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
-    const int nq = rq.T * G;
-    if (q0 >= nq) return;
+    if (rq.over && kvh == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+    const int nq = rq.T * G;   // at most NQ
+    if (nq == 0) return;
     int SL;
     const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
     if (split >= ns) return;
-    // visible tokens of the chunk's last query end this CTA's range
-    const int p0 = split * SL, p1 = min(p0 + SL, rq.pos + (min(q0 + NQ, nq) - 1) / G + 1);
+    const int p0 = split * SL, p1 = min(p0 + SL, rq.kvlen);
 
-    // blocks and scales of the split: {block (-1: outside the cache), K scale, V scale, its logarithm}
-    float4 *pages = reinterpret_cast<float4 *>(sm + 4 * FEW_STAGES * STAGE);
+    // blocks (-1: outside the cache) of the split, then their {K scale, V scale, its logarithm}
     const int e0 = p0 / bs, ne = p1 > p0 ? (p1 - 1) / bs - e0 + 1 : 0;
+    int *page_id = reinterpret_cast<int *>(sm + 4 * FEW_STAGES * STAGE);
+    float4 *page = reinterpret_cast<float4 *>(page_id + a.pages);
+    const int *trow = a.table + (size_t)r * a.max_blocks + e0;
     for (int i = tid; i < ne; i += 128) {
-        const int b = a.table[(size_t)r * a.max_blocks + e0 + i];
-        float4 e = make_float4(__int_as_float(-1), 0.0f, 0.0f, -INFINITY);
-        if (b >= 0 && b < a.kv.n_blocks) {
-            const size_t bh = (size_t)b * KH + kvh;
-            e.x = __int_as_float(b);
-            e.y = a.kv.k_scale[bh];
-            e.z = a.kv.v_scale[bh];
-            e.w = lg2(e.z);
-        } else {
+        int b = trow[i];
+        if (b < 0 || b >= a.kv.n_blocks) {
+            b = -1;
             vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
         }
-        pages[i] = e;
+        page_id[i] = b;
+    }
+
+    // pieces w, w + 4, ... of 32 tokens: 2 tiles each
+    const int npc = p1 > p0 ? (p1 - p0 + 31) >> 5 : 0, nit = npc > w ? (npc - w + 3) >> 2 : 0;
+    unsigned char *ring = sm + w * (FEW_STAGES * STAGE);
+    const uint32_t ring_u = smem_u32(ring);
+    const int bs16 = bs >> 4;
+    const uint8_t *kb = (const uint8_t *)a.kv.k + (size_t)kvh * bs * HD + lane * 16;
+    const uint8_t *vb = (const uint8_t *)a.kv.v + (size_t)kvh * bs * HD + lane * 16;
+    const size_t bstep = (size_t)KH * bs * HD;
+    const int tile0 = p0 / 16 - e0 * bs16 + 2 * w;   // the warp's first tile, counted from the first page's start
+    int pi = tile0 / bs16, oi = tile0 % bs16;        // page and tile in it of the next tile to bring in
+    int pc = pi, oc = oi;                            // and of the next one to use
+    int p_in = p0 + 32 * w;
+    __syncthreads();   // page_id
+    auto issue = [&](int it) {
+        if (it < nit) {
+            uint32_t dst = ring_u + it % FEW_STAGES * STAGE;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int blk = p_in < p1 ? page_id[pi] : -1;
+                const size_t at = (size_t)max(blk, 0) * bstep + (size_t)(oi * 16) * HD;
+                const uint8_t *ks = kb + at, *vs = vb + at;
+                const int live = blk >= 0 ? rq.kvlen - p_in : 0;   // tokens of the tile that exist
+                // instruction k brings chunks 32 k + lane of the span
+                auto bring = [&](auto copy) {
+#pragma unroll
+                    for (int k = 0; k < HD / 32; k++) {
+                        const int byte = k * 512 + lane * 16, row = byte / HD, in = byte % HD;
+                        copy(dst + P::k_slot(row, in), ks + k * 512, row);
+                        copy(dst + HD * 16 + P::v_slot(row, in), vs + k * 512, row);
+                    }
+                };
+                if (live >= 16) bring([](uint32_t d, const uint8_t *x, int) { cp_async<16>(d, x); });
+                else bring([&](uint32_t d, const uint8_t *x, int row) { cp_async_zfill<16>(d, x, row < live); });
+                dst += TILE;
+                p_in += 16;
+                oi += u == 0 ? 1 : 7;   // the pair's second tile; the warp's next piece
+                while (oi >= bs16) oi -= bs16, pi++;
+            }
+            p_in += 96;
+        }
+        cp_commit();
+    };
+    if (nit > 0) {
+#pragma unroll 1
+        for (int i = 0; i < FEW_STAGES - 1; i++) issue(i);
+    }
+    for (int i = tid; i < ne; i += 128) {
+        const int b = page_id[i];
+        float4 e = make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
+        if (b >= 0) {
+            const size_t bh = (size_t)b * KH + kvh;
+            e.x = a.kv.k_scale[bh];
+            e.y = a.kv.v_scale[bh];
+            e.z = lg2(e.y);
+        }
+        page[i] = e;
     }
 
     // queries: fragments hi (and lo), the factor of each row's scores
@@ -118,7 +176,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     int lim[NR];   // last visible token
 #pragma unroll
     for (int i = 0; i < NR; i++) {
-        const int q = q0 + g + 8 * i;
+        const int q = g + 8 * i;
         const bool have = q < nq;
         const int row = rq.row0 + (have ? q / G : 0), h = kvh * G + (have ? q % G : 0);
         const float *x = a.q + (size_t)row * a.ldq + (size_t)h * HD;
@@ -157,52 +215,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < NR; i++) m[i] = mv[i] = -INFINITY, l[i] = 0.0f;
 
-    // pieces w, w + 4, ... of the range
-    const int npc = p1 > p0 ? (p1 - p0 + 31) >> 5 : 0, nit = npc > w ? (npc - w + 3) >> 2 : 0;
-    unsigned char *ring = sm + w * (FEW_STAGES * STAGE);
-    const uint32_t ring_u = smem_u32(ring);
-    const int bs16 = bs >> 4;
-    const uint8_t *kb = (const uint8_t *)a.kv.k + (size_t)kvh * bs * HD + lane * 16;
-    const uint8_t *vb = (const uint8_t *)a.kv.v + (size_t)kvh * bs * HD + lane * 16;
-    const size_t bstep = (size_t)KH * bs * HD;
-    const int tile0 = p0 / 16 - e0 * bs16 + 2 * w;   // the warp's first tile, counted from the first page's start
-    int pi = tile0 / bs16, oi = tile0 % bs16;        // page and tile in it of the next tile to bring in
-    int pc = pi, oc = oi;                            // and of the next one to use
-    int p_in = p0 + 32 * w;
-    __syncthreads();   // pages
-    auto issue = [&](int it) {
-        if (it < nit) {
-            uint32_t dst = ring_u + it % FEW_STAGES * STAGE;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int blk = p_in < p1 ? __float_as_int(pages[pi].x) : -1;
-                const size_t at = (size_t)max(blk, 0) * bstep + (size_t)(oi * 16) * HD;
-                const uint8_t *ks = kb + at, *vs = vb + at;
-                const int live = blk >= 0 ? rq.kvlen - p_in : 0;   // tokens of the tile that exist
-                // instruction k brings chunks 32 k + lane of the span
-                auto bring = [&](auto copy) {
-#pragma unroll
-                    for (int k = 0; k < HD / 32; k++) {
-                        const int byte = k * 512 + lane * 16, row = byte / HD, in = byte % HD;
-                        copy(dst + P::k_slot(row, in), ks + k * 512, row);
-                        copy(dst + HD * 16 + P::v_slot(row, in), vs + k * 512, row);
-                    }
-                };
-                if (live >= 16) bring([](uint32_t d, const uint8_t *x, int) { cp_async<16>(d, x); });
-                else bring([&](uint32_t d, const uint8_t *x, int row) { cp_async_zfill<16>(d, x, row < live); });
-                dst += TILE;
-                p_in += 16;
-                oi += u == 0 ? 1 : 7;   // the pair's second tile; the warp's next piece
-                while (oi >= bs16) oi -= bs16, pi++;
-            }
-            p_in += 96;
-        }
-        cp_commit();
-    };
-    if (nit > 0) {
-#pragma unroll 1
-        for (int i = 0; i < FEW_STAGES - 1; i++) issue(i);
-    }
+    __syncthreads();   // page
 #pragma unroll 1
     for (int it = 0; it < nit; it++) {
         __syncwarp();   // every lane has read the piece that is replaced
@@ -216,9 +229,10 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         bool none[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const float4 e = p0 + 32 * (w + 4 * it) + 16 * u < p1 ? pages[pc] : make_float4(__int_as_float(-1), 0.f, 0.f, -INFINITY);
-            none[u] = __float_as_int(e.x) < 0;
-            ksc[u] = e.y, vsc[u] = e.z, lv[u] = e.w;
+            const bool in = p0 + 32 * (w + 4 * it) + 16 * u < p1;
+            const float4 e = in ? page[pc] : make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
+            none[u] = !in || page_id[pc] < 0;
+            ksc[u] = e.x, vsc[u] = e.y, lv[u] = e.z;
             oc += u == 0 ? 1 : 7;
             while (oc >= bs16) oc -= bs16, pc++;
 #pragma unroll
@@ -382,8 +396,10 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         }
     }
     __syncthreads();
-    // one warp per query
-    for (int q = w; q < NQ && q0 + q < nq; q += 4) {
+    // the CTA's result, one warp per query: {m, l, -, -, o[HD]}, unnormalised
+    const bool cluster = a.S <= 8;
+    float *res = sml + 4 * NQ * 2;                        // [NQ][HD + 4]
+    for (int q = w; q < nq; q += 4) {
         float M = -INFINITY, mw[4], L = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) M = fmaxf(M, mw[k] = sml[(k * NQ + q) * 2]);
@@ -392,8 +408,8 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
             mw[k] = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
             L += mw[k] * sml[(k * NQ + q) * 2 + 1];
         }
-        const int row = rq.row0 + (q0 + q) / G, h = kvh * G + (q0 + q) % G;
-        float *rec = a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
+        const int row = rq.row0 + q / G, h = kvh * G + q % G;
+        float *rec = cluster ? res + q * (HD + 4) : a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
         float *out = a.out + (size_t)row * a.ldo + (size_t)h * HD;
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
 #pragma unroll
@@ -407,6 +423,33 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         }
         if (ns > 1 && lane == 0) *reinterpret_cast<float2 *>(rec) = make_float2(M, L);
     }
+    if (!cluster || ns == 1) return;
+    // every CTA of the cluster that got here has ns splits: they share out the queries
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (int q = split + ns * w; q < nq; q += 4 * ns) {
+        float M = -INFINITY, L = 0.0f, mw[8], x[HD / 32];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < ns) M = fmaxf(M, mw[k] = *cl.map_shared_rank(res + q * (HD + 4), k));
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) x[d] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k < ns) {
+                const float *rec = cl.map_shared_rank(res + q * (HD + 4), k);
+                const float e = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
+                L = fmaf(e, rec[1], L);
+#pragma unroll
+                for (int d = 0; d < HD / 32; d++) x[d] = fmaf(e, rec[4 + d * 32 + lane], x[d]);
+            }
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        float *out = a.out + (size_t)(rq.row0 + q / G) * a.ldo + (size_t)(kvh * G + q % G) * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) out[d * 32 + lane] = x[d] * inv;
+    }
+    cl.sync();   // the others have read this CTA's results
 }
 
 // Joins the splits of the requests that have several: one warp per (row, head).
@@ -471,9 +514,9 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
 // How a call is cut: kernel, queries per CTA and splits.
 struct AttnPlan {
     int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), KV8_TILE_Q (k_kv8_attn_many)
-    int chunks;    // chunks per (request, kv head) at most, or tiles of all requests
+    int tiles;     // k_kv8_attn_many: tiles of all requests at most
     int S, sl_min;
-    int sl_max;    // tokens of a split at most
+    int pages;     // blocks a split may touch (k_kv8_attn_few)
 };
 #ifndef ATTN_FEW_MAX
 #define ATTN_FEW_MAX 16   // queries of a request and kv head up to which k_kv8_attn_few is used
@@ -487,15 +530,24 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
     long long units, S;
     if (most <= ATTN_FEW_MAX) {
         p.nq = most <= 8 ? 8 : 16;
-        p.chunks = (int)((most + p.nq - 1) / p.nq);
-        p.sl_min = 256;
-        // two rounds of CTAs on the GPU when every request has a full table
-        units = (long long)n_req * kv->n_kv_heads * (p.chunks > 0 ? p.chunks : 1);
-        S = (2 * 148 * 3 + units - 1) / units;
+        p.tiles = 0;
+        units = (long long)n_req * kv->n_kv_heads;
+        // A CTA costs about 3.5 us besides its tokens (1.4 us for 128), two fit an SM.  So: as many
+        // splits as fit the GPU at once, none shorter than the cost warrants (128 tokens for a few
+        // units, 1024 for 256 of them); more only to even out long contexts (4096 tokens).  Measured:
+        // 256 units of 768 tokens 13.5 us whole, 17.5 in two; 264 units of up to 16384 162 us whole,
+        // 122 in four, 152 in eight; 32 units of 768 9.2 us whole, 7.3 in six.
+        const long long wide = units / 32 < 1 ? 1 : units / 32 > 32 ? 32 : units / 32;
+        p.sl_min = (int)(128 * wide);
+        S = 2 * 148 / units;
+        const long long even = (tokens + 4095) / 4096;
+        // above 8 a second kernel joins the splits: worth it for long ones only
+        if (S > 8 && tokens <= 8 * 512) S = 8;
+        if (S < even) S = even;
     } else {
         p.nq = KV8_TILE_Q;
         const long long full = (long long)n_rows * G / KV8_TILE_Q;
-        p.chunks = (int)(full + n_req);
+        p.tiles = (int)(full + n_req);
         p.sl_min = 512;
         const long long busy = n_req < n_rows ? n_req : n_rows;
         units = (full > busy ? full : busy) * kv->n_kv_heads;
@@ -503,21 +555,26 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
     }
     const long long need = (tokens + p.sl_min - 1) / p.sl_min;
     if (S > need) S = need;
-    if (S > 64) S = 64;
     // k_kv8_attn_few: a tensor core's sums lose up to an ulp per step: 8192 tokens are 128 steps per
     // warp, 5e-6 at most
-    if (p.nq < KV8_TILE_Q && S < (tokens + 8191) / 8192) S = (tokens + 8191) / 8192;
+    const long long least = p.nq < KV8_TILE_Q ? (tokens + 8191) / 8192 : 1;
+    if (S > 64) S = 64;
+    if (S < least) S = least;
     p.S = (int)(S < 1 ? 1 : S);
-    const long long even = (tokens + p.S - 1) / p.S;
-    p.sl_max = (int)(((even > p.sl_min ? even : p.sl_min) + 127) & ~127ll);
+    // tokens of a split at most (kv8_splits)
+    const long long even = (tokens + p.S - 1) / p.S, sl_max = ((even > p.sl_min ? even : p.sl_min) + 127) & ~127ll;
+    p.pages = (int)(sl_max / kv->block_size + 2 + 3) & ~3;
     return p;
 }
+
+// Whether the splits leave records for k_kv8_attn_join.
+static bool attn_records(const AttnPlan &p) { return p.S > (p.nq == KV8_TILE_Q ? 1 : 8); }
 
 extern "C" size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new,
                                                int max_blocks) {
     if (attn_check(kv, n_heads, n_req, n_rows, max_new, max_blocks)) return 0;
     const AttnPlan p = attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks);
-    return p.S > 1 ? (size_t)n_rows * n_heads * p.S * (kv->head_dim + 4) * sizeof(float) : 0;
+    return attn_records(p) ? (size_t)n_rows * n_heads * p.S * (kv->head_dim + 4) * sizeof(float) : 0;
 }
 
 typedef void (*attn_kernel_t)(const Kv8AttnArgs);
@@ -567,18 +624,19 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
     if (n_rows == 0) return 0;
     const int hd = kv->head_dim;
     const Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, n_req, n_rows, max_new,
-                           out, ldo, (float *)workspace, p.S, p.sl_min, vxc_device_error_ptr()};
+                           out, ldo, (float *)workspace, p.S, p.sl_min, p.pages, vxc_device_error_ptr()};
     if (p.nq == KV8_TILE_Q) {
-        VXC_CUDA_OK(kv8_attn_many(a, p.chunks, (cudaStream_t)stream));
+        VXC_CUDA_OK(kv8_attn_many(a, p.tiles, (cudaStream_t)stream));
     } else {
         attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
-        size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)(p.sl_max / kv->block_size + 2) * sizeof(float4);
-        const size_t join = (size_t)4 * p.nq * (hd + 6) * sizeof(float);
+        size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)p.pages * (sizeof(int) + sizeof(float4));
+        const size_t join = ((size_t)4 * p.nq * (hd + 6) + (size_t)p.nq * (hd + 4)) * sizeof(float);
         if (smem < join) smem = join;
         VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
-        VXC_CUDA_OK(kv8_launch(f, dim3(kv->n_kv_heads * p.chunks, p.S, n_req), dim3(128), smem, (cudaStream_t)stream, 1, a));
+        VXC_CUDA_OK(kv8_launch(f, dim3(p.S, kv->n_kv_heads, n_req), dim3(128), smem, (cudaStream_t)stream,
+                               p.S <= 8 ? p.S : 1, a));
     }
-    if (p.S > 1)
+    if (attn_records(p))
         VXC_CUDA_OK(kv8_launch(join_kernel(hd), dim3(n_rows, (n_heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, 1, a));
     return 0;
 }

@@ -19,6 +19,7 @@ struct Kv8AttnArgs {
     long long ldo;
     float *part;        // records of the splits
     int S, sl_min;      // splits per request at most, tokens per split at least
+    int pages;          // blocks a split may touch, rounded up to 4 (k_kv8_attn_few)
     unsigned int *err;
 };
 
