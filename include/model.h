@@ -24,6 +24,12 @@
  *                   gets the full logits.  Destroy speculative states that
  *                   use such a model before the model: their CUDA graphs
  *                   hold the model's NCCL operations.
+ * vx_model_set_kv_cache (additive) how the model's KV cache is held from its
+ *                   next forward on: 0 fp32 (as created), VXC_KV8_INT8 (1) or
+ *                   VXC_KV8_E4M3 (2) the paged 8-bit cache of
+ *                   include/veltrix_cuda.h.  The present cache is dropped and
+ *                   cache_len set to 0.  Speculative states keep fp32 caches
+ *                   of their own.  VX_ERR_PARAM for another type.
  */
 #ifndef VX_MODEL_H
 #define VX_MODEL_H
@@ -39,6 +45,7 @@ void vx_model_destroy(vx_model *model);
 vx_error vx_model_forward(vx_model *model, const int *tokens, int n_tokens, float *logits);
 int vx_model_generate_greedy(vx_model *model, const int *prompt, int n_prompt, int *out, int max_tokens,
                              int eos_id);
+vx_error vx_model_set_kv_cache(vx_model *model, int type);
 vx_error vx_model_create_tp(const char *path, int rank, int world, const void *nccl_id, vx_model **model);
 
 #ifdef __cplusplus

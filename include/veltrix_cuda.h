@@ -189,6 +189,18 @@ size_t vxc_net_weight_bytes(const vxc_net *net);
  * one [layer][n_ctx][kv_dim] cache per model) plus work buffers for up to
  * max_rows rows per forward call. */
 int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_rows, vxc_seqs **out);
+/* The same with the KV cache held in 8 bits and in blocks (vxc_kv8, below):
+ * kv_type VXC_KV8_INT8 or VXC_KV8_E4M3, n_blocks blocks of block_size tokens
+ * per layer for all slots together (0: enough for max_ctx positions in every
+ * slot).  A forward gives a slot the blocks its positions need and takes back
+ * those behind them; with fewer blocks than every slot's context needs, a
+ * forward that finds none free raises the device error word and caches
+ * nothing.  One forward takes one group per slot (a second one is left out and
+ * raises the error word; n_groups <= n_slots).  n_slots <= VXC_KV8_MAX_REQ.
+ * vxc_forward, vxc_forward_host and vxc_greedy_generate use either kind;
+ * logits differ from the fp32 cache's by the rounding of K and V to 8 bits. */
+int vxc_seqs_create_kv8(const vxc_net *net, int n_slots, int max_ctx, int max_rows, int kv_type, int block_size,
+                        int n_blocks, vxc_seqs **out);
 void vxc_seqs_destroy(vxc_seqs *s);
 
 /* Batched forward (reference vx_model_forward, src/model.c:391-628, for many

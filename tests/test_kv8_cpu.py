@@ -82,6 +82,15 @@ def test_without_a_device_every_call_is_unsupported():
     assert tables() == UNSUPPORTED
 
 
+def test_sequence_set_and_model_refusals():
+    L = vxb200.lib()
+    h = ctypes.c_void_p()
+    assert L.vxc_seqs_create_kv8(None, 1, 64, 64, 1, 64, 0, ctypes.byref(h)) == PARAM
+    for kind, nb in ((0, 0), (3, 0), (1, -1)):
+        assert L.vxc_seqs_create_kv8(BUF, 1, 64, 64, kind, 64, nb, ctypes.byref(h)) == PARAM
+    assert L.vx_model_set_kv_cache(None, 1) == PARAM
+
+
 # ---- the restatement itself ---------------------------------------------------
 
 def test_e4m3_codes_against_torch():

@@ -261,13 +261,12 @@ def test_attn_lengths_beyond_the_arguments_are_reported(cuda, new):
 def test_attn_workspace_too_small_is_refused(cuda):
     import vxb200
     d = Dev(cuda, INT8, 70, 64, 1, 128)
-    size = d.c.attn_workspace_bytes(8, 1, 1, 1, 64)
-    if size == 0:
-        pytest.skip("these sizes need no workspace")
+    size = d.c.attn_workspace_bytes(8, 1, 1, 1, 400)
+    assert size > 0
     x = cuda.zeros(4096, device="cuda")
     p = x.data_ptr()
     for ws, n in ((p, size - 1), (None, size)):
-        rc = vxb200.lib().vxc_kv8_attn(d.c.ref, p, 1024, 8, 0.1, p, 64, p, p, 1, 1, 1, p, 1024, ws, n, None)
+        rc = vxb200.lib().vxc_kv8_attn(d.c.ref, p, 1024, 8, 0.1, p, 400, p, p, 1, 1, 1, p, 1024, ws, n, None)
         assert rc == -4 and b"workspace" in vxb200.lib().vxc_error_string()
 
 

@@ -105,3 +105,14 @@ int vxc_net_world(const vxc_net *n);
 int vxc_tp_world(const vxc_tp *t);
 int vxc_tp_allreduce_sum(const vxc_tp *t, float *buf, size_t n, cudaStream_t st);
 int vxc_tp_allgather(const vxc_tp *t, const float *send, float *recv, size_t n, cudaStream_t st);
+
+// The paged 8-bit KV cache in the forward (vxc_kv8.cu, vxc_kv8_attn.cu): block
+// tables without a slot map; attention of n_groups groups of rows_per_group
+// rows, group g at position d_pos[g] with table row d_seq[g] (negative: left
+// out), q and out rows of n_heads x head_dim floats.
+int vxc_kv8_check(const vxc_kv8 *kv, const char *who);
+int vxc_kv8_tables_only(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks, int max_blocks,
+                        int *d_table, int *d_held, int *d_free, int *d_state, int *d_row0, cudaStream_t st);
+int vxc_kv8_attn_groups(const vxc_kv8 *kv, const float *q, int n_heads, float scale, const int *d_table, int max_blocks,
+                        const int *d_seq, const int *d_pos, int n_groups, int rows_per_group, float *out, void *workspace,
+                        size_t workspace_bytes, cudaStream_t st);

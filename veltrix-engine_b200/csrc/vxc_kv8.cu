@@ -103,10 +103,12 @@ __device__ __forceinline__ int tb_find(const int *a, int n, int i) {
     return lo;
 }
 
+// (No __restrict__ here or below: a load through a const restricted pointer is
+// taken for one of constant data, and may be moved above griddepcontrol.wait.)
 __global__ void __launch_bounds__(TB_THREADS)
-    k_kv8_tables(const int *__restrict__ d_len, const int *__restrict__ d_new, int n, int bs, int nb, int max_blocks,
-                 int *__restrict__ table, int *__restrict__ d_held, int *__restrict__ ring, int *__restrict__ state,
-                 int n_rows, int *__restrict__ d_row0, int *__restrict__ d_slot, unsigned int *err) {
+    k_kv8_tables(const int *d_len, const int *d_new, int n, int bs, int nb, int max_blocks,
+                 int *table, int *d_held, int *ring, int *state,
+                 int n_rows, int *d_row0, int *d_slot, unsigned int *err) {
     extern __shared__ int sm[];
     int *row0 = sm, *pop0 = row0 + n + 1, *push0 = pop0 + n + 1, *held = push0 + n + 1;   // held[n]
     __shared__ int wsum[3][32], carry[3];
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(TB_THREADS)
     const int gt = blockIdx.x * TB_THREADS + tid, gs = gridDim.x * TB_THREADS;
     if (status) {
         for (int i = gt; i <= n; i += gs) d_row0[i] = 0;
-        for (int i = gt; i < n_rows; i += gs) d_slot[i] = -1;
+        for (int i = gt; d_slot && i < n_rows; i += gs) d_slot[i] = -1;
         if (gt == 0) {
             state[2] = status;
             if (status > 1) vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(TB_THREADS)
         state[2] = 0;
     }
     const int total = (int)t_new;
-    for (int i = gt; i < n_rows; i += gs) {
+    for (int i = gt; d_slot && i < n_rows; i += gs) {
         int s = -1;
         if (i < total) {
             const int r = tb_find(row0, n, i);
@@ -278,6 +280,18 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
     return 0;
 }
 
+// The forward's form: no slot map, any number of rows (sizes checked when the
+// sequence set was made).
+int vxc_kv8_tables_only(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks, int max_blocks,
+                        int *d_table, int *d_held, int *d_free, int *d_state, int *d_row0, cudaStream_t st) {
+    const size_t smem = (size_t)(4 * n_req + 3) * sizeof(int);
+    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (4 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
+    VXC_CUDA_OK(kv8_launch(k_kv8_tables, dim3(1), dim3(TB_THREADS), smem, st, 1, d_len, d_new, n_req, block_size, n_blocks,
+                           max_blocks, d_table, d_held, d_free, d_state, INT_MAX, d_row0, (int *)NULL,
+                           vxc_device_error_ptr()));
+    return 0;
+}
+
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
@@ -301,8 +315,8 @@ __device__ __forceinline__ void team_sync(int team) {
 
 template <int TYPE, int TS>
 __global__ void __launch_bounds__(AP_THREADS, 4)
-    k_kv8_append(const vxc_kv8 kv, const float *__restrict__ kx, long long ldk, const float *__restrict__ vx,
-                 long long ldv, const int *__restrict__ slot, int n_rows, int window, int lsh, int units, unsigned int *err) {
+    k_kv8_append(const vxc_kv8 kv, const float *kx, long long ldk, const float *vx,
+                 long long ldv, const int *slot, int n_rows, int window, int lsh, int units, unsigned int *err) {
     constexpr int TEAMS = AP_THREADS / TS;
     extern __shared__ int sm[];
     __shared__ float red[AP_THREADS / 32];

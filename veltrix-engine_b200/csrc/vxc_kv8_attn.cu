@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     const int e0 = p0 / bs, ne = p1 > p0 ? (p1 - 1) / bs - e0 + 1 : 0;
     int *page_id = reinterpret_cast<int *>(sm + 4 * FEW_STAGES * STAGE);
     float4 *page = reinterpret_cast<float4 *>(page_id + a.pages);
-    const int *trow = a.table + (size_t)r * a.max_blocks + e0;
+    const int *trow = rq.table + e0;
     for (int i = tid; i < ne; i += 128) {
         int b = trow[i];
         if (b < 0 || b >= a.kv.n_blocks) {
@@ -459,11 +459,11 @@ __global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
     pdl_trigger();
     pdl_wait();
     const int i = blockIdx.x, h = blockIdx.y * 4 + w;
-    if (h >= a.H || i >= a.row0[a.n_req]) return;
+    if (h >= a.H || i >= kv8_row0(a, a.n_req)) return;
     int lo = 0, hi = a.n_req;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a.row0[mid] <= i) lo = mid; else hi = mid;
+        if (kv8_row0(a, mid) <= i) lo = mid; else hi = mid;
     }
     const Kv8Req rq = kv8_req(a, lo);
     if (i - rq.row0 < 0 || i - rq.row0 >= rq.T) return;
@@ -598,6 +598,31 @@ static attn_kernel_t join_kernel(int hd) {
     }
 }
 
+// The launches of a call whose arguments hold.
+static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st) {
+    Kv8AttnArgs a = args;
+    a.S = p.S;
+    a.sl_min = p.sl_min;
+    a.pages = p.pages;
+    a.err = vxc_device_error_ptr();
+    const vxc_kv8 *kv = &a.kv;
+    const int hd = kv->head_dim;
+    if (p.nq == KV8_TILE_Q) {
+        VXC_CUDA_OK(kv8_attn_many(a, p.tiles, st));
+    } else {
+        attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
+        size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)p.pages * (sizeof(int) + sizeof(float4));
+        const size_t join = ((size_t)4 * p.nq * (hd + 6) + (size_t)p.nq * (hd + 4)) * sizeof(float);
+        if (smem < join) smem = join;
+        VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
+        VXC_CUDA_OK(kv8_launch(f, dim3(p.S, kv->n_kv_heads, a.n_req), dim3(128), smem, st,
+                               p.S <= 8 ? p.S : 1, a));
+    }
+    if (attn_records(p))
+        VXC_CUDA_OK(kv8_launch(join_kernel(hd), dim3(a.n_rows, (a.H + 3) / 4), dim3(128), 0, st, 1, a));
+    return 0;
+}
+
 extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, int n_heads, float scale,
                             const int *d_table, int max_blocks, const int *d_row0, const int *d_pos, int n_req,
                             int n_rows, int max_new, float *out, long long ldo, void *workspace,
@@ -622,21 +647,24 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
     }
     if (int rc = vxc_require_device()) return rc;
     if (n_rows == 0) return 0;
-    const int hd = kv->head_dim;
-    const Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, n_req, n_rows, max_new,
-                           out, ldo, (float *)workspace, p.S, p.sl_min, p.pages, vxc_device_error_ptr()};
-    if (p.nq == KV8_TILE_Q) {
-        VXC_CUDA_OK(kv8_attn_many(a, p.tiles, (cudaStream_t)stream));
-    } else {
-        attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
-        size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)p.pages * (sizeof(int) + sizeof(float4));
-        const size_t join = ((size_t)4 * p.nq * (hd + 6) + (size_t)p.nq * (hd + 4)) * sizeof(float);
-        if (smem < join) smem = join;
-        VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
-        VXC_CUDA_OK(kv8_launch(f, dim3(p.S, kv->n_kv_heads, n_req), dim3(128), smem, (cudaStream_t)stream,
-                               p.S <= 8 ? p.S : 1, a));
+    const Kv8AttnArgs a = {*kv, q, ldq, n_heads, scale, d_table, max_blocks, d_row0, d_pos, NULL, n_req, n_rows, max_new,
+                           out, ldo, (float *)workspace};
+    return attn_run(a, p, (cudaStream_t)stream);
+}
+
+// The forward's form: n_groups groups of rows_per_group rows, group g at
+// position d_pos[g] with the blocks of table row d_seq[g] (none if negative).
+int vxc_kv8_attn_groups(const vxc_kv8 *kv, const float *q, int n_heads, float scale, const int *d_table, int max_blocks,
+                        const int *d_seq, const int *d_pos, int n_groups, int rows_per_group, float *out, void *workspace,
+                        size_t workspace_bytes, cudaStream_t st) {
+    const int rows = n_groups * rows_per_group, width = n_heads * kv->head_dim;
+    if (int rc = attn_check(kv, n_heads, n_groups, rows, rows_per_group, max_blocks)) return rc;
+    const AttnPlan p = attn_plan(kv, n_heads, n_groups, rows, rows_per_group, max_blocks);
+    if (vxc_kv8_attn_workspace_bytes(kv, n_heads, n_groups, rows, rows_per_group, max_blocks) > workspace_bytes) {
+        vxc_set_error("vxc_forward: attention workspace too small");
+        return -4;
     }
-    if (attn_records(p))
-        VXC_CUDA_OK(kv8_launch(join_kernel(hd), dim3(n_rows, (n_heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, 1, a));
-    return 0;
+    const Kv8AttnArgs a = {*kv, q, width, n_heads, scale, d_table, max_blocks, NULL, d_pos, d_seq, n_groups, rows,
+                           rows_per_group, out, width, (float *)workspace};
+    return attn_run(a, p, st);
 }

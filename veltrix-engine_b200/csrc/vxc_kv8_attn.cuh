@@ -12,8 +12,9 @@ struct Kv8AttnArgs {
     float scale;
     const int *table;
     int max_blocks;
-    const int *row0;    // [n_req + 1]
+    const int *row0;    // [n_req + 1], or NULL: max_new rows each
     const int *pos;     // [n_req]
+    const int *seq;     // NULL, or the table row of each request (negative: the request has no rows)
     int n_req, n_rows, max_new;
     float *out;
     long long ldo;
@@ -84,20 +85,23 @@ __device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &h01, uint32_t &h2
 
 // A request's rows and tokens as the call's arguments and arrays allow them.
 struct Kv8Req {
+    const int *table;
     int row0, T;     // first row; rows (clamped to n_rows, max_new and the table)
     int pos;         // position of the first row
     int kvlen;       // tokens the last row sees (0: none)
     bool over;       // something was clamped
 };
+__device__ __forceinline__ int kv8_row0(const Kv8AttnArgs &a, int r) { return a.row0 ? a.row0[r] : r * a.max_new; }
 __device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
     Kv8Req q;
-    const int r0 = a.row0[r], r1 = a.row0[r + 1];
+    const int r0 = kv8_row0(a, r), s = a.seq ? a.seq[r] : r, r1 = s < 0 ? r0 : kv8_row0(a, r + 1);
+    q.table = a.table + (size_t)max(s, 0) * a.max_blocks;
     q.pos = a.pos[r];
     q.row0 = max(r0, 0);
     long long T = (long long)r1 - r0;
     const long long cap = (long long)a.max_blocks * a.kv.block_size;
     const long long most = min(min((long long)a.max_new, (long long)a.n_rows - q.row0), cap - q.pos);
-    q.over = r0 < 0 || T > most;
+    q.over = r0 < 0 || (T > 0 && T > most);
     T = r0 < 0 ? 0 : min(T, most);
     q.T = (int)max(T, 0ll);
     q.kvlen = q.T > 0 ? max(q.pos + q.T, 0) : 0;

@@ -123,12 +123,12 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         int hi = a.n_req;
         while (hi - r > 1) {
             const int mid = (r + hi) >> 1;
-            if ((long long)max(a.row0[mid], 0) * G / KV8_TILE_Q + mid <= idx) r = mid; else hi = mid;
+            if ((long long)max(kv8_row0(a, mid), 0) * G / KV8_TILE_Q + mid <= idx) r = mid; else hi = mid;
         }
     }
     const Kv8Req rq = kv8_req(a, r);
     const long long tile0 = (long long)rq.row0 * G / KV8_TILE_Q + r;
-    if (kvh == 0 && split == 0 && tid == 0 && ((rq.over && idx == tile0) || (idx == 0 && a.row0[a.n_req] > a.n_rows)))
+    if (kvh == 0 && split == 0 && tid == 0 && ((rq.over && idx == tile0) || (idx == 0 && kv8_row0(a, a.n_req) > a.n_rows)))
         vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
     const int nq = rq.T * G;
     const long long q0l = (idx - tile0) * KV8_TILE_Q;
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         } else if (warp == 18 && lane < 8) {
             // ------------------------------ blocks and scales ------------------------------
-            const int *trow = a.table + (size_t)r * a.max_blocks;
+            const int *trow = rq.table;
             for (int j = 0; j < nt; j++) {
                 const int e = j % MN_PAGES;
                 if (j >= MN_PAGES && !mn_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI)) break;

@@ -16,7 +16,8 @@
 // does (freq = 1/powf(theta, 2i/hd), val = pos*freq, cosf/sinf), and the
 // rotation is written with explicitly rounded ops, so it matches the
 // reference bit-for-bit.  The KV cache is fp32, head-major
-// ([layer][slot][kv head][pos][hd]).
+// ([layer][slot][kv head][pos][hd]), or, for a sequence set made by
+// vxc_seqs_create_kv8, the paged 8-bit cache of vxc_kv8.cu.
 //
 // Weights are Q4_0/Q8_0 (tensor-core GEMV, vxc_gemv_tc.cu) or K-quant
 // (CUDA-core GEMV on the same activation image, vxc_kquant.cu).  Under tensor
@@ -84,6 +85,18 @@ struct vxc_seqs {
     uint64_t tmk[16], tmv[16];   // CUtensorMap of the K and V caches as [rows][hd] (copied to an aligned local per launch)
     float *ar;               // [max_rows][E] all-reduced projection output (tensor parallel)
     float *lg_local, *lg_all;   // local logits [rows][Vl], gathered [world][rows][Vl]
+    // paged 8-bit cache (kv8.type 0: the fp32 cache above); kv8 describes layer 0, layer l begins
+    // l x n_blocks blocks behind it
+    vxc_kv8 kv8;
+    int max_blocks;          // blocks per table row
+    int *i8;                 // the int arrays below, one allocation
+    int *table, *held, *ring, *state, *row0;   // vxc_kv8_tables over the slots
+    int *len, *fresh;        // per slot: cached tokens before the call, new ones
+    int *seq, *tok_slot;     // per group: table row or -1; per row: cache slot or -1
+    float *krow, *vrow;      // [max_rows][kv dim] new K and V rows
+    float *arow;             // [max_rows][H hd] attention output
+    void *kv8_ws;
+    size_t kv8_ws_bytes;
 };
 
 // queries per attention CTA: 8 when a kv head has <= 8 queries (verify rows x
@@ -185,11 +198,12 @@ __device__ __forceinline__ float block_max(float v, float *red) {
 
 // RoPE of one head of row m (qkv = sum of the fused QKV GEMV's partials):
 // blockIdx.x < H: q head -> qbuf; < H + KH: k head -> cache; else v head ->
-// cache (head-major [slot][kv head][pos][hd]).  Thread = one (even, odd) pair.
+// cache (head-major [slot][kv head][pos][hd]), or to row m of kc and vc when
+// to_rows (the paged cache's append reads them).  Thread = one (even, odd) pair.
 __global__ void k_rope_kv(Part qkv, int T, const int *__restrict__ d_slot, const int *__restrict__ d_pos,
                           const float2 *__restrict__ rope, int max_pos, int H, int KH, int hd,
                           float *__restrict__ qbuf, float *__restrict__ kc, float *__restrict__ vc, int n_slots,
-                          int max_ctx, unsigned int *err) {
+                          int max_ctx, int to_rows, unsigned int *err) {
     pdl_trigger();
     pdl_wait();
     const int head = blockIdx.x, m = blockIdx.y, p = threadIdx.x;
@@ -202,7 +216,9 @@ __global__ void k_rope_kv(Part qkv, int T, const int *__restrict__ d_slot, const
         return;
     }
     if (2 * p >= hd) return;
-    auto cache_row = [&](float *c, int kh) { return c + (((size_t)slot * KH + kh) * max_ctx + pos) * hd; };
+    auto cache_row = [&](float *c, int kh) {
+        return to_rows ? c + ((size_t)m * KH + kh) * hd : c + (((size_t)slot * KH + kh) * max_ctx + pos) * hd;
+    };
     if (head >= H + KH) {
         const int vh = head - H - KH;
         float *dst = cache_row(vc, vh) + 2 * p;
@@ -678,6 +694,92 @@ __global__ void __launch_bounds__(ROW_THREADS) k_combine_image(const float *__re
         image_cols(img, chunk_bytes, csh, m, M, h0 * hd, h1 * hd, s, [&](int k) { return v[k - h0 * hd]; });
     }
     cl.sync();
+}
+
+// The paged cache's row kernels.  (No __restrict__: a load through a const
+// restricted pointer may be moved above griddepcontrol.wait, and k_kv8_rows then
+// read the state of the tables before they were made.)
+// Row m of x[M][W] (W = H hd) as the operand of the attention-output GEMV: the
+// paged cache's attention writes finished rows.
+__global__ void __launch_bounds__(ROW_THREADS) k_rows_image(const float *x, int W, int M,
+                                                              uint8_t *img, size_t chunk_bytes, int csh,
+                                                              float *xs, float *xf) {
+    extern __shared__ float v[];
+    __shared__ float red[32], slots[1];
+    cg::cluster_group cl = cg::this_cluster();
+    pdl_trigger();
+    pdl_wait();
+    const int m = blockIdx.y;
+    int k0, k1;
+    col_range(W, 8, &k0, &k1);
+    float mx = 0.0f;
+    for (int i = k0 + threadIdx.x; i < k1; i += blockDim.x) {
+        const float a = x[(size_t)m * W + i];
+        v[i - k0] = a;
+        if (!img) xf[(size_t)m * W + i] = a;
+        mx = fmaxf(mx, fabsf(a));
+    }
+    if (img) {
+        mx = cluster_reduce(cl, block_max(mx, red), &slots[0], 1);
+        const float s = vxc_prescale(mx);
+        if (blockIdx.x == 0 && threadIdx.x == 0) xs[m] = s;
+        __syncthreads();
+        image_cols(img, chunk_bytes, csh, m, M, k0, k1, s, [&](int k) { return v[k - k0]; });
+    }
+    cl.sync();
+}
+
+// Lengths for vxc_kv8_tables from a forward's groups (one CTA): a slot with a
+// group has pos[g] tokens before it and min(T, max_ctx - pos[g]) new ones, any
+// other slot keeps its blocks.  seq[g] = the group's slot, or -1 for a slot or
+// position outside the set (k_rope_kv reports it) and for the second group of
+// one slot (reported here: their order would decide the tables).
+__global__ void __launch_bounds__(1024) k_kv8_groups(const int *d_slot, const int *d_pos,
+                                                       int n_groups, int T, int n_slots, int max_ctx, int bs,
+                                                       const int *held, int *len,
+                                                       int *fresh, int *seq,
+                                                       unsigned int *err) {
+    extern __shared__ int owner[];   // [n_slots] first group of a slot
+    pdl_trigger();
+    pdl_wait();
+    for (int s = threadIdx.x; s < n_slots; s += blockDim.x) owner[s] = INT_MAX;
+    __syncthreads();
+    auto valid = [&](int g) { return d_slot[g] >= 0 && d_slot[g] < n_slots && d_pos[g] >= 0 && d_pos[g] < max_ctx; };
+    for (int g = threadIdx.x; g < n_groups; g += blockDim.x)
+        if (valid(g)) atomicMin(&owner[d_slot[g]], g);
+    __syncthreads();
+    for (int g = threadIdx.x; g < n_groups; g += blockDim.x) {
+        const bool mine = valid(g) && owner[d_slot[g]] == g;
+        seq[g] = mine ? d_slot[g] : -1;
+        if (valid(g) && !mine) vxc_flag_error(err, VXC_DERR_BAD_SHAPE);
+    }
+    for (int s = threadIdx.x; s < n_slots; s += blockDim.x) {
+        const int g = owner[s];
+        len[s] = g < INT_MAX ? d_pos[g] : held[s] * bs;
+        fresh[s] = g < INT_MAX ? min(T, max_ctx - d_pos[g]) : 0;
+    }
+}
+
+// Cache slot of every row of the forward after its tables: -1 for rows that are
+// left out, and for all rows when the tables could not be made (no free blocks:
+// the error word gets CTX_FULL).
+__global__ void k_kv8_rows(const int *seq, const int *d_pos, int M, int T, int max_ctx, int bs,
+                           int max_blocks, int n_blocks, const int *table, const int *state,
+                           int *tok_slot, unsigned int *err) {
+    pdl_trigger();
+    pdl_wait();
+    const int m = blockIdx.x * blockDim.x + threadIdx.x;
+    const bool ok = state[2] == 0;
+    if (m == 0 && !ok) vxc_flag_error(err, VXC_DERR_CTX_FULL);
+    if (m >= M) return;
+    const int s = seq[m / T];
+    int to = -1;
+    if (ok && s >= 0) {
+        const int p = d_pos[m / T] + m % T;
+        const int b = p < max_ctx ? table[(size_t)s * max_blocks + p / bs] : -1;
+        if (b >= 0 && b < n_blocks) to = b * bs + p % bs;
+    }
+    tok_slot[m] = to;
 }
 
 // logits[m][w*Vl + v] = gathered[w][m][v]: the vocabulary shards of the GPUs side by side
@@ -1330,7 +1432,9 @@ static size_t part_slot_floats(const vxc_net *n) {
     return (best + 63) & ~(size_t)63;
 }
 
-extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_rows, vxc_seqs **out) {
+// kv_type 0: the fp32 cache; else the paged 8-bit cache.
+static int seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_rows, int kv_type, int block_size,
+                       int n_blocks, vxc_seqs **out) {
     if (!net || !out || n_slots <= 0 || max_ctx <= 0 || max_rows <= 0) { vxc_set_error("vxc_seqs_create: bad args"); return -4; }
     int rc = vxc_require_device();
     if (rc) return rc;
@@ -1345,6 +1449,30 @@ extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int
     // this GPU's share under tensor parallelism (everything when net->tp == NULL)
     const int E = c.n_embd, kvd = net->KHl * c.n_head_dim, F = net->Fl, hd = c.n_head_dim;
     const int nch = (max_rows + 63) / 64;
+    if (kv_type) {
+        // as many blocks as every slot's context needs, unless told otherwise
+        const int per = (max_ctx + (block_size > 0 ? block_size : 1) - 1) / (block_size > 0 ? block_size : 1);
+        const long long nb = n_blocks > 0 ? n_blocks : (long long)n_slots * per;
+        s->kv8 = {kv_type, (int)(nb < INT_MAX ? nb : INT_MAX), block_size, net->KHl, hd, NULL, NULL, NULL, NULL};
+        s->max_blocks = per;
+        // (the arrays are allocated below; a stand-in address lets the sizes be checked first)
+        s->kv8.k = s->kv8.v = (void *)256;
+        s->kv8.k_scale = s->kv8.v_scale = (float *)256;
+        rc = n_slots > VXC_KV8_MAX_REQ ? -4 : vxc_kv8_check(&s->kv8, "vxc_seqs_create_kv8");
+        if (n_slots > VXC_KV8_MAX_REQ) vxc_set_error("vxc_seqs_create_kv8: %d slots (at most %d)", n_slots, VXC_KV8_MAX_REQ);
+        if (rc) {
+            free(s);
+            return rc;
+        }
+        // attention scratch: the most any shape of a forward needs
+        for (int g = 1; g <= n_slots && g <= max_rows; g++)
+            for (int t = 1; (long long)g * t <= max_rows; t++) {
+                const size_t b = vxc_kv8_attn_workspace_bytes(&s->kv8, net->Hl, g, g * t, t, per);
+                if (b > s->kv8_ws_bytes) s->kv8_ws_bytes = b;
+            }
+        s->kv8.k = s->kv8.v = NULL;
+        s->kv8.k_scale = s->kv8.v_scale = NULL;
+    }
     size_t kvn = (size_t)c.n_layers * n_slots * max_ctx * kvd;
     // attention split length: at most 16 splits of >= ATTN_SL_MIN positions (whole
     // tiles).  Short splits and a 2-stage ring keep ~5 CTAs per SM resident, which
@@ -1355,13 +1483,28 @@ extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int
     if (SL < sl_min) SL = sl_min;
     s->attn_sl = SL;
     s->attn_splits = (max_ctx + SL - 1) / SL;
-    size_t part = (size_t)max_rows * net->Hl * s->attn_splits * (hd + 4);
+    size_t part = kv_type ? 0 : (size_t)max_rows * net->Hl * s->attn_splits * (hd + 4);
     s->img_chunk = (size_t)(E > F ? E : F) / 32 * vxc_img_block_bytes(64);
     s->part_slot = part_slot_floats(net);
     cudaError_t e = cudaSuccess;
 #define ALLOC(p, n) if (e == cudaSuccess) e = cudaMalloc((void **)&(p), (n))
-    ALLOC(s->k, kvn * 4);
-    ALLOC(s->v, kvn * 4);
+    const size_t n8 = (size_t)c.n_layers * s->kv8.n_blocks * net->KHl, b8 = n8 * block_size * hd;   // scales, codes
+    const size_t i8 = (size_t)n_slots * s->max_blocks + 5 * (size_t)n_slots + s->kv8.n_blocks + 2 * (size_t)max_rows + 8;
+    if (kv_type) {
+        ALLOC(s->kv8.k, b8);
+        ALLOC(s->kv8.v, b8);
+        ALLOC(s->kv8.k_scale, n8 * 4);
+        ALLOC(s->kv8.v_scale, n8 * 4);
+        ALLOC(s->i8, i8 * 4);
+        ALLOC(s->krow, (size_t)max_rows * kvd * 4);
+        ALLOC(s->vrow, (size_t)max_rows * kvd * 4);
+        ALLOC(s->arow, (size_t)max_rows * net->Hl * hd * 4);
+        if (s->kv8_ws_bytes) ALLOC(s->kv8_ws, s->kv8_ws_bytes);
+    } else {
+        ALLOC(s->k, kvn * 4);
+        ALLOC(s->v, kvn * 4);
+        ALLOC(s->attn_part, part * 4);
+    }
     ALLOC(s->x, (size_t)max_rows * E * 4);
     ALLOC(s->qbuf, (size_t)max_rows * E * 4);
     ALLOC(s->img, (size_t)nch * s->img_chunk);
@@ -1372,29 +1515,55 @@ extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int
         if ((size_t)net->Hl * hd > kmax) kmax = (size_t)net->Hl * hd;
         ALLOC(s->xf, (size_t)VXC_SKINNY_MAX_M * kmax * 4);
     }
-    ALLOC(s->attn_part, part * 4);
     if (net->tp) {
         ALLOC(s->ar, (size_t)max_rows * E * 4);
         ALLOC(s->lg_local, (size_t)max_rows * net->Vl * 4);
         ALLOC(s->lg_all, (size_t)net->world * max_rows * net->Vl * 4);
     }
 #undef ALLOC
-    if (e == cudaSuccess) e = cudaMemset(s->k, 0, kvn * 4);
-    if (e == cudaSuccess) e = cudaMemset(s->v, 0, kvn * 4);
+    if (kv_type) {
+        // empty scales and tables, every block free
+        std::vector<int> h(i8, 0);
+        s->table = s->i8;
+        s->held = s->table + (size_t)n_slots * s->max_blocks;
+        s->row0 = s->held + n_slots;
+        s->len = s->row0 + n_slots + 1;
+        s->fresh = s->len + n_slots;
+        s->state = s->fresh + n_slots;
+        s->ring = s->state + 3;
+        s->seq = s->ring + s->kv8.n_blocks;
+        s->tok_slot = s->seq + max_rows;
+        for (size_t i = 0; i < (size_t)n_slots * s->max_blocks; i++) h[i] = -1;
+        h[s->state - s->i8 + 1] = s->kv8.n_blocks;
+        for (int b = 0; b < s->kv8.n_blocks; b++) h[s->ring - s->i8 + b] = b;
+        if (e == cudaSuccess) e = cudaMemcpy(s->i8, h.data(), i8 * 4, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaMemset(s->kv8.k, 0, b8);
+        if (e == cudaSuccess) e = cudaMemset(s->kv8.v, 0, b8);
+        if (e == cudaSuccess) e = cudaMemset(s->kv8.k_scale, 0, n8 * 4);
+        if (e == cudaSuccess) e = cudaMemset(s->kv8.v_scale, 0, n8 * 4);
+        // rows of groups that are left out stay as they were: never NaN
+        if (e == cudaSuccess) e = cudaMemset(s->arow, 0, (size_t)max_rows * net->Hl * hd * 4);
+        if (e == cudaSuccess) e = cudaMemset(s->krow, 0, (size_t)max_rows * kvd * 4);
+        if (e == cudaSuccess) e = cudaMemset(s->vrow, 0, (size_t)max_rows * kvd * 4);
+        if (e == cudaSuccess) e = cudaMemset(s->qbuf, 0, (size_t)max_rows * E * 4);
+    } else {
+        if (e == cudaSuccess) e = cudaMemset(s->k, 0, kvn * 4);
+        if (e == cudaSuccess) e = cudaMemset(s->v, 0, kvn * 4);
+    }
     if (e == cudaSuccess) e = cudaMemset(s->img, 0, (size_t)nch * s->img_chunk);
     if (e == cudaSuccess && !attn_kernel(hd, 16)) {
         vxc_set_error("vxc_seqs_create: head dim %d not supported (32, 64, 96 or 128)", hd);
         vxc_seqs_destroy(s);
         return -7;
     }
-    if (e == cudaSuccess && attn_smem(hd, SL, ATTN_QC_MAX) > 227 * 1024) {
+    if (e == cudaSuccess && !kv_type && attn_smem(hd, SL, ATTN_QC_MAX) > 227 * 1024) {
         vxc_set_error("vxc_seqs_create: context %d too long for the attention split", max_ctx);
         vxc_seqs_destroy(s);
         return -4;
     }
     // the attention kernel addresses cache rows with 32-bit tensor-map coordinates
     const uint64_t kv_rows = (uint64_t)c.n_layers * n_slots * net->KHl * max_ctx;
-    if (e == cudaSuccess && (kv_rows + ATTN_T >= (1ull << 31) || !attn_tmap(s->k, hd, kv_rows, s->tmk) ||
+    if (e == cudaSuccess && !kv_type && (kv_rows + ATTN_T >= (1ull << 31) || !attn_tmap(s->k, hd, kv_rows, s->tmk) ||
                              !attn_tmap(s->v, hd, kv_rows, s->tmv))) {
         vxc_set_error("vxc_seqs_create: no tensor map for a KV cache of %llu rows of %d", (unsigned long long)kv_rows, hd);
         vxc_seqs_destroy(s);
@@ -1410,7 +1579,7 @@ extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int
     // must not shrink it under one with a longer context.
     static const int attn_qcs[] = {1, 2, 3, 4, 5, 6, 7, 8, 16};
     for (int qc : attn_qcs) {
-        if (e != cudaSuccess) break;
+        if (e != cudaSuccess || kv_type) break;
         cudaFuncAttributes fa;
         const int need = (int)attn_smem(hd, SL, qc);
         e = cudaFuncGetAttributes(&fa, attn_kernel(hd, qc));
@@ -1426,9 +1595,23 @@ extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int
     return 0;
 }
 
+extern "C" int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_rows, vxc_seqs **out) {
+    return seqs_create(net, n_slots, max_ctx, max_rows, 0, 0, 0, out);
+}
+
+extern "C" int vxc_seqs_create_kv8(const vxc_net *net, int n_slots, int max_ctx, int max_rows, int kv_type,
+                                   int block_size, int n_blocks, vxc_seqs **out) {
+    if ((kv_type != VXC_KV8_INT8 && kv_type != VXC_KV8_E4M3) || n_blocks < 0) {
+        vxc_set_error("vxc_seqs_create_kv8: cache type %d, %d blocks", kv_type, n_blocks);
+        return -4;
+    }
+    return seqs_create(net, n_slots, max_ctx, max_rows, kv_type, block_size, n_blocks, out);
+}
+
 extern "C" void vxc_seqs_destroy(vxc_seqs *s) {
     if (!s) return;
-    void *ptrs[] = {s->k, s->v, s->x, s->qbuf, s->img, s->xs, s->part, s->xf, s->attn_part, s->ar, s->lg_local,
+    void *ptrs[] = {s->kv8.k, s->kv8.v, s->kv8.k_scale, s->kv8.v_scale, s->i8, s->krow, s->vrow, s->arow, s->kv8_ws,
+                    s->k, s->v, s->x, s->qbuf, s->img, s->xs, s->part, s->xf, s->attn_part, s->ar, s->lg_local,
                     s->lg_all};
     for (void *p : ptrs)
         if (p) cudaFree(p);
@@ -1575,6 +1758,10 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
         vxc_set_error("vxc_forward: %d rows exceed max_rows %d", M, s->max_rows);
         return -4;
     }
+    if (s->kv8.type && n_groups > s->n_slots) {
+        vxc_set_error("vxc_forward: %d groups for %d slots (a paged cache takes one group per slot)", n_groups, s->n_slots);
+        return -4;
+    }
     const vxc_net *n = s->net;
     const vxc_net_config &c = n->cfg;
     // heads, kv heads and FFN columns of this GPU (all of them without tensor parallelism)
@@ -1615,6 +1802,21 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
     e = launch_pdl(k_embed, dim3(M), dim3(256), 0, st, n->embd, n->embd_type, n->embd_row_bytes,
                                n->embd_rows, E, d_tokens, s->x, err);
     prof_end(0, pe, st);
+    if (s->kv8.type && e == cudaSuccess) {
+        // blocks for the new tokens, and where each row's token goes
+        const vxc_kv8 &kv = s->kv8;
+        e = launch_pdl(k_kv8_groups, dim3(1), dim3(1024), (size_t)s->n_slots * sizeof(int), st, d_slot, d_pos, n_groups, T,
+                       s->n_slots, s->max_ctx < c.max_pos ? s->max_ctx : c.max_pos, kv.block_size, (const int *)s->held,
+                       s->len, s->fresh, s->seq, err);
+        if (e == cudaSuccess) {
+            if ((rc = vxc_kv8_tables_only(s->len, s->fresh, s->n_slots, kv.block_size, kv.n_blocks, s->max_blocks, s->table,
+                                          s->held, s->ring, s->state, s->row0, st)))
+                return rc;
+            e = launch_pdl(k_kv8_rows, dim3(nblk(M, 256)), dim3(256), 0, st, (const int *)s->seq, d_pos, M, T, s->max_ctx,
+                           kv.block_size, s->max_blocks, kv.n_blocks, (const int *)s->table, (const int *)s->state,
+                           s->tok_slot, err);
+        }
+    }
     const int G = H / KH, nq = T * G, qcn = attn_qc(nq), nqc = (nq + qcn - 1) / qcn;
     const size_t asm_bytes = attn_smem(hd, s->attn_sl, qcn);
     CUtensorMap tmk, tmv;
@@ -1625,6 +1827,7 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
     size_t row_smem = (size_t)cols8(E);
     if ((size_t)cols8(F) > row_smem) row_smem = cols8(F);
     if ((size_t)((H + ROW_CL - 1) / ROW_CL) * hd > row_smem) row_smem = (size_t)((H + ROW_CL - 1) / ROW_CL) * hd;
+    if ((size_t)cols8(H * hd) > row_smem) row_smem = cols8(H * hd);
     row_smem *= sizeof(float);
     Part prev;
     prev.base = NULL;
@@ -1647,8 +1850,9 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
     static_assert(VXC_GEMM_SLAB == 256, "slab rows = 2^8");
     for (int l = 0; l < c.n_layers && e == cudaSuccess; l++) {
         const vxc_layer_dev *d = &n->layers[l];
-        float *kc = s->k + (size_t)l * s->n_slots * s->max_ctx * kvd;
-        float *vc = s->v + (size_t)l * s->n_slots * s->max_ctx * kvd;
+        const bool paged = s->kv8.type != 0;
+        float *kc = paged ? s->krow : s->k + (size_t)l * s->n_slots * s->max_ctx * kvd;
+        float *vc = paged ? s->vrow : s->v + (size_t)l * s->n_slots * s->max_ctx * kvd;
         pe = prof_begin(st);
         ImgOut io = img_for(d->wqkv, M);
         e = launch_pdl_cluster(k_norm_image, dim3(ROW_CL, M), dim3(ROW_THREADS), row_smem, st, ROW_CL, s->x, prev,
@@ -1660,18 +1864,35 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
         prof_end(2, pe, st);
         pe = prof_begin(st);
         e = launch_pdl(k_rope_kv, dim3(H + 2 * KH, M), dim3(((hd / 2) + 31) / 32 * 32), 0, st, pp, T, d_slot, d_pos, (const float2 *)n->rope,
-                       c.max_pos, H, KH, hd, s->qbuf, kc, vc, s->n_slots, s->max_ctx, err);
+                       c.max_pos, H, KH, hd, s->qbuf, kc, vc, s->n_slots, s->max_ctx, paged ? 1 : 0, err);
+        vxc_kv8 kv = s->kv8;
+        if (paged) {   // this layer's blocks
+            const size_t skip = (size_t)l * kv.n_blocks * KH;
+            kv.k = (uint8_t *)kv.k + skip * kv.block_size * hd;
+            kv.v = (uint8_t *)kv.v + skip * kv.block_size * hd;
+            kv.k_scale += skip;
+            kv.v_scale += skip;
+            if (e == cudaSuccess && (rc = vxc_kv8_append(&kv, s->krow, kvd, s->vrow, kvd, s->tok_slot, M, stream))) return rc;
+        }
         prof_end(3, pe, st);
         if (e != cudaSuccess) break;
         pe = prof_begin(st);
-        e = launch_pdl(attn_kernel(hd, qcn), dim3(n_groups * KH * nqc, s->attn_splits), dim3(128), asm_bytes, st,
+        if (paged) {
+            if ((rc = vxc_kv8_attn_groups(&kv, s->qbuf, H, 1.0f / sqrtf((float)hd), s->table, s->max_blocks, s->seq, d_pos,
+                                          n_groups, T, s->arow, s->kv8_ws, s->kv8_ws_bytes, st)))
+                return rc;
+        } else e = launch_pdl(attn_kernel(hd, qcn), dim3(n_groups * KH * nqc, s->attn_splits), dim3(128), asm_bytes, st,
                        (const float *)s->qbuf, T, d_slot, d_pos, H, KH, tmk, tmv, l * s->n_slots * KH * s->max_ctx,
                        s->n_slots, s->max_ctx, s->attn_sl, nqc, s->attn_part, err);
         prof_end(4, pe, st);
         if (e != cudaSuccess) break;
         pe = prof_begin(st);
         io = img_for(d->wo, M);
-        e = launch_pdl_cluster(k_combine_image, dim3(ROW_CL, M), dim3(ROW_THREADS), row_smem, st, ROW_CL,
+        if (paged)
+            e = launch_pdl_cluster(k_rows_image, dim3(ROW_CL, M), dim3(ROW_THREADS), row_smem, st, ROW_CL,
+                                   (const float *)s->arow, H * hd, M, io.img, io.bytes, io.csh, s->xs, s->xf);
+        else
+            e = launch_pdl_cluster(k_combine_image, dim3(ROW_CL, M), dim3(ROW_THREADS), row_smem, st, ROW_CL,
                                (const float *)s->attn_part, T, H, KH, hd, s->attn_splits, M, io.img, io.bytes,
                                io.csh, s->xs, s->xf);
         prof_end(5, pe, st);

@@ -255,12 +255,26 @@ static vx_error ensure_seqs(vxb_model *m) {
     vxc_net_config nc;
     vxc_net_config_get(m->net, &nc);
     if (ctx > nc.max_pos) return VX_ERR_PARAM;
-    if (vxc_seqs_create(m->net, 1, ctx, VXB_CHUNK_ROWS, &m->seqs) != 0) {
+    if ((m->kv_type ? vxc_seqs_create_kv8(m->net, 1, ctx, VXB_CHUNK_ROWS, m->kv_type, VXB_KV8_BLOCK, 0, &m->seqs)
+                    : vxc_seqs_create(m->net, 1, ctx, VXB_CHUNK_ROWS, &m->seqs)) != 0) {
         fprintf(stderr, "veltrix-b200: %s\n", vxc_error_string());
         return VX_ERR_MEMORY;
     }
     m->seqs_ctx = ctx;
     m->pub.cache_len = 0;
+    return VX_OK;
+}
+
+vx_error vx_model_set_kv_cache(vx_model *model, int type) {
+    if (!model || (type != 0 && type != VXC_KV8_INT8 && type != VXC_KV8_E4M3)) return VX_ERR_PARAM;
+    vxb_model *m = vxb_of(model);
+    if (m->kv_type != type) {
+        if (m->seqs && vxc_device_current() != m->device) vxc_device_init(m->device);
+        vxc_seqs_destroy(m->seqs);
+        m->seqs = NULL;
+        m->kv_type = type;
+    }
+    model->cache_len = 0;
     return VX_OK;
 }
 

@@ -48,6 +48,8 @@ PROTOTYPES = {
     "vxc_net_config_get": (ctypes.c_int, [_vp, _vp]),
     "vxc_net_weight_bytes": (ctypes.c_size_t, [_vp]),
     "vxc_seqs_create": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
+    "vxc_seqs_create_kv8": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                           ctypes.c_int, ctypes.POINTER(_vp)]),
     "vxc_seqs_destroy": (None, [_vp]),
     "vxc_forward": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp, _vp]),
     "vxc_forward_host": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp]),
@@ -56,6 +58,7 @@ PROTOTYPES = {
     "vx_model_create_tp": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, _vp, ctypes.POINTER(_vp)]),
     "vx_model_destroy": (None, [_vp]),
     "vx_model_forward": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp]),
+    "vx_model_set_kv_cache": (ctypes.c_int, [_vp, ctypes.c_int]),
     "vx_model_generate_greedy": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int]),
     "vxc_greedy_generate": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int,
                                            ctypes.c_int, _c_int_p, _c_int_p]),
@@ -256,6 +259,12 @@ class Model:
         if rc != 0:
             raise VxError(f"vx_model_forward = {rc}: {lib().vxc_error_string()}")
         return out
+
+    def set_kv_cache(self, ctype):
+        """vx_model_set_kv_cache: 0 fp32, KV8_INT8 or KV8_E4M3; drops what is cached."""
+        rc = lib().vx_model_set_kv_cache(self.h, ctype)
+        if rc != 0:
+            raise VxError(f"vx_model_set_kv_cache = {rc}")
 
     def generate_greedy(self, prompt, max_tokens, eos_id=-1):
         """vx_model_generate_greedy: the emitted tokens (int32 array)."""
