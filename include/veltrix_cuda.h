@@ -306,7 +306,7 @@ typedef struct {
  * go to its back, in request and table order, and their entries become -1.
  * The queue is the ring d_free[n_blocks] with d_state = {front, count,
  * status}; a block put back by a call can be taken by the next one.
- * (max_blocks * block_size <= 2^30.)  d_table,
+ * (max_blocks * block_size and n_rows are at most 2^30.)  d_table,
  * d_held, d_free and d_state are updated in place.
  * Outputs: d_row0[n_req + 1], the first row of each request's new tokens and
  * their total, and d_slot[n_rows], the slot of every new token, request after

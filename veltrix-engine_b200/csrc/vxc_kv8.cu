@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(TB_THREADS)
                  int *table, int *d_held, int *ring, int *state,
                  int n_rows, int *d_row0, int *d_slot, unsigned int *err) {
     extern __shared__ int sm[];
-    int *row0 = sm, *pop0 = row0 + n + 1, *push0 = pop0 + n + 1, *held = push0 + n + 1;   // held[n]
+    int *row0 = sm, *pop0 = row0 + n + 1, *push0 = pop0 + n + 1;
+    int *held = push0 + n + 1, *lens = held + n;   // [n]
     __shared__ int wsum[3][32], carry[3];
     __shared__ long long tot[4][32];
     __shared__ int wbad[32];
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(TB_THREADS)
                 }
             }
             held[r] = h;
+            lens[r] = len;
         }
         // inclusive scan of the three counts over the CTA (wrapping: totals are checked in 64 bits)
 #pragma unroll
@@ -221,7 +223,10 @@ __global__ void __launch_bounds__(TB_THREADS)
         d_row0[r] = row0[r];
         if (r < n) d_held[r] = held[r] + (pop0[r + 1] - pop0[r]) - (push0[r + 1] - push0[r]);
     }
-    auto ring_at = [&](long long i) -> int & { return ring[(head + i) % nb]; };
+    auto ring_at = [&](long long i) -> int & {   // i <= n_blocks
+        const long long at = head + i;
+        return ring[at >= nb ? at - nb : at];
+    };
     for (int i = gt; i < (int)t_more; i += gs) {
         const int r = tb_find(pop0, n, i), b = ring_at(i);
         table[(size_t)r * max_blocks + held[r] + (i - pop0[r])] = b;
@@ -238,18 +243,30 @@ __global__ void __launch_bounds__(TB_THREADS)
         state[1] = (int)(count - t_more + t_less);
         state[2] = 0;
     }
+    // four rows at a time, so that their loads are under way together
     const int total = (int)t_new;
-    for (int i = gt; d_slot && i < n_rows; i += gs) {
-        int s = -1;
-        if (i < total) {
-            const int r = tb_find(row0, n, i);
-            const unsigned p = (unsigned)d_len[r] + (unsigned)(i - row0[r]);
-            const int j = (int)(p / (unsigned)bs);
-            const int b = j < held[r] ? table[(size_t)r * max_blocks + j] : ring_at((long long)pop0[r] + j - held[r]);
-            if (b >= 0 && b < nb) s = b * bs + (int)(p % (unsigned)bs);
-            else vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
+    for (int i0 = gt; d_slot && i0 < n_rows; i0 += 4 * gs) {
+        int b[4], off[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * gs;
+            b[k] = off[k] = -1;
+            if (i < total) {
+                const int r = tb_find(row0, n, i);
+                const unsigned p = (unsigned)lens[r] + (unsigned)(i - row0[r]);
+                const int j = (int)(p / (unsigned)bs);
+                off[k] = (int)(p - (unsigned)j * (unsigned)bs);
+                b[k] = j < held[r] ? table[(size_t)r * max_blocks + j] : ring_at((long long)pop0[r] + j - held[r]);
+            }
         }
-        d_slot[i] = s;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * gs;
+            if (i >= n_rows) break;
+            const bool ok = b[k] >= 0 && b[k] < nb;
+            if (!ok && i < total) vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
+            d_slot[i] = ok ? b[k] * bs + off[k] : -1;
+        }
     }
 }
 
@@ -260,7 +277,7 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
         vxc_set_error("vxc_kv8_tables: an array is missing");
         return -4;
     }
-    if (n_req < 1 || n_req > VXC_KV8_MAX_REQ || n_rows < 0) {
+    if (n_req < 1 || n_req > VXC_KV8_MAX_REQ || n_rows < 0 || n_rows > KV8_MAX_TOKENS) {
         vxc_set_error("vxc_kv8_tables: %d requests (1 to %d), %d rows", n_req, VXC_KV8_MAX_REQ, n_rows);
         return -4;
     }
@@ -270,10 +287,10 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
         return -4;
     }
     if (int rc = vxc_require_device()) return rc;
-    const size_t smem = (size_t)(4 * n_req + 3) * sizeof(int);
+    const size_t smem = (size_t)(5 * n_req + 3) * sizeof(int);
     const int nc = n_rows >= TB_CLUSTER_ROWS ? TB_CLUSTER : 1;
     // the static arrays take the rest of the default 48 KB
-    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (4 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
+    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (5 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
     VXC_CUDA_OK(kv8_launch(k_kv8_tables, dim3(nc), dim3(TB_THREADS), smem, (cudaStream_t)stream, nc, d_len, d_new,
                            n_req, block_size, n_blocks, max_blocks, d_table, d_held, d_free, d_state, n_rows, d_row0,
                            d_slot, vxc_device_error_ptr()));
@@ -284,8 +301,8 @@ extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int
 // sequence set was made).
 int vxc_kv8_tables_only(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks, int max_blocks,
                         int *d_table, int *d_held, int *d_free, int *d_state, int *d_row0, cudaStream_t st) {
-    const size_t smem = (size_t)(4 * n_req + 3) * sizeof(int);
-    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (4 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
+    const size_t smem = (size_t)(5 * n_req + 3) * sizeof(int);
+    if (smem > 44 * 1024) VXC_CUDA_OK(kv8_allow_smem((const void *)k_kv8_tables, (5 * VXC_KV8_MAX_REQ + 3) * sizeof(int)));
     VXC_CUDA_OK(kv8_launch(k_kv8_tables, dim3(1), dim3(TB_THREADS), smem, st, 1, d_len, d_new, n_req, block_size, n_blocks,
                            max_blocks, d_table, d_held, d_free, d_state, INT_MAX, d_row0, (int *)NULL,
                            vxc_device_error_ptr()));
