@@ -100,6 +100,11 @@ __device__ __forceinline__ bool mn_wait(uint32_t bar, uint32_t parity, volatile 
 // The softmax warps only.
 __device__ __forceinline__ void mn_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// Every warp, at the end of its role.  Registers go back to what the block was launched with only behind
+// this: a warp that is done early (one has nothing to do at all) would otherwise take back registers that a
+// softmax warp has not got yet, and that warp would wait for them for ever.
+__device__ __forceinline__ void mn_roles_done() { asm volatile("bar.sync 2, %0;" ::"n"(MN_THREADS) : "memory"); }
+
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnArgs a) {
     using M = MnSmem<HD>;
@@ -237,7 +242,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         }
         cp_wait<0>();
         __syncwarp();
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");   // what the block was launched with, for the code behind the roles
+        mn_roles_done();
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     } else if (warp < MN_LOADERS / 32 + 8) {
         // ------------------------------ softmax ------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
@@ -444,6 +450,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        mn_roles_done();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 16 && lane == 0) {
@@ -517,6 +524,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         }
         __syncwarp();
+        mn_roles_done();
         asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     }
 
