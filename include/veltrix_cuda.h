@@ -294,7 +294,7 @@ typedef struct {
     int n_blocks, block_size;       /* block_size a multiple of 16, 16..256 */
     int n_kv_heads, head_dim;       /* head_dim 32, 64, 96 or 128 */
     void *k, *v;                    /* [n_blocks][n_kv_heads][block_size][head_dim] bytes */
-    float *k_scale, *v_scale;       /* [n_blocks][n_kv_heads], zero at first */
+    float *k_scale, *v_scale;       /* [n_blocks][n_kv_heads], zero at first; never negative */
 } vxc_kv8;
 
 /* Block tables and slot maps from request lengths.  Request r (r < n_req <=

@@ -27,11 +27,25 @@
 //                Weights of tile j first, then O of tile j - 1 is added, so its
 //                product runs beside them
 //   warp 16      issues S of tile j + 2; warp 17 issues P V of tile j
-//   warp 18      block table and scales of the coming tiles
+//   warp 18      block table and scales of the coming tiles, four at a time
+//   warp 19      nothing: registers are shared out by fours of warps
 // TMEM: two buffers of 128 columns for S / P, 128 for O, 128 for Q.
 // K and V tiles have two slots each.  K as [head dim chunk][token] x 16 bytes
 // is K-major, V in the same layout is MN-major; chunks are 2064 bytes apart, so
-// the loaders' 16-byte stores fall into different banks.
+// the loaders' 16-byte stores fall into different banks.  Queries and outputs
+// go through shared memory, 16 columns at a time, so that an instruction
+// touches 8 lines instead of 32 (queries read a lane per row: 5 us a CTA).
+//
+// Measured (32 query heads of 128 over 8 kv heads): 8192 rows behind 8192
+// tokens of one request 3.43 ms, 561 Tflop/s of attention = 1.12 Pflop/s of
+// fp16 products, 68 % of what a dense bf16 product reaches; 8 prompts of 512
+// rows 122 us; 32 requests of 7 rows behind 4096 tokens 150 us (28 of a tile's
+// 128 queries exist).  Bound: the softmax warps' instructions (scores are read,
+// multiplied, exponentiated, split in two and stored), tensor pipe busy half of
+// the time.  Slower: one thread per query, -9 %; each half of the softmax
+// warps on a tile of its own, -5 to -10 %; persistent CTAs over a list of
+// tiles, -20 %; 128 loader threads; queries in shared memory; warps that skip
+// their arithmetic when none of their queries exist, -6 %.
 // Every wait is bounded (VXC_WAIT_NS); on expiry the error word is set, every
 // role leaves its loop, and TMEM is freed after the issued work has ended.
 #include "vxc_kv8_attn.cuh"
@@ -46,8 +60,8 @@ template <int HD>
 struct MnSmem {
     static constexpr int TILE = HD / 8 * MN_CHUNK;          // one fp16 tile of 128 rows
     static constexpr int PIECE = 128 * (HD == 96 ? 128 : HD);   // raw bytes of one (96: as 8 units per row)
-    static constexpr int K = 0, V = 2 * TILE, RAW = 4 * TILE, BYTES = RAW + MN_AHEAD * PIECE;
-    static_assert(4 * TILE >= (129 * HD + 512) * 4, "the join's [HD][129] and [128][4] floats lie in the K and V slots");
+    static constexpr int STAGED = 32 * 20 * 4;                  // a softmax warp's 32 rows x 16 columns, 20 floats a row
+    static constexpr int K = 0, V = 2 * TILE, RAW = 4 * TILE, OUT = RAW + MN_AHEAD * PIECE, BYTES = OUT + 8 * STAGED;
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
@@ -97,6 +111,10 @@ __device__ __forceinline__ bool mn_wait(uint32_t bar, uint32_t parity, volatile 
     return mbar_try(bar, parity) || mbar_wait(bar, parity, abort_flag, err, code);
 }
 
+// The factor of a group's scores, kept above 0: a masked score (-inf) times it is -inf, never NaN.
+// (Where it would be less, a score is below 1e-25 either way: the weight is the same.)
+__device__ __forceinline__ float mn_factor(float x) { return fmaxf(x, 1e-37f); }
+
 // The softmax warps only.
 __device__ __forceinline__ void mn_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -124,12 +142,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     // every request as many as it needs; later tiles (longer contexts) first
     const int idx = (int)gridDim.x - 1 - (int)blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
     int r = 0;
-    {
-        int hi = a.n_req;
-        while (hi - r > 1) {
-            const int mid = (r + hi) >> 1;
-            if ((long long)max(kv8_row0(a, mid), 0) * G / KV8_TILE_Q + mid <= idx) r = mid; else hi = mid;
-        }
+    for (int len = a.n_req; len > 1;) {   // 32 places a step
+        const int step = (len + 31) / 32, at = lane * step;
+        const bool le = at < len && (long long)max(kv8_row0(a, r + at), 0) * G / KV8_TILE_Q + r + at <= idx;
+        const unsigned mask = __ballot_sync(0xffffffffu, le);
+        const int k = mask ? 31 - __clz(mask) : 0;
+        r += k * step;
+        len = min(step, len - k * step);
     }
     const Kv8Req rq = kv8_req(a, r);
     const long long tile0 = (long long)rq.row0 * G / KV8_TILE_Q + r;
@@ -251,21 +270,37 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         const int half = (warp >> 2) - MN_LOADERS / 128, row = tid & 127;
         const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
         const int q = q0 + row;
+        // Global rows are read and written 16 columns at a time, 4 lanes a row (a lane per row would touch
+        // 32 lines an instruction), and change hands in the warp's own space: lane = row there.
+        float *st = reinterpret_cast<float *>(sm + M::OUT + (warp - MN_LOADERS / 32) * M::STAGED);
+        const int wrow = (warp & 3) * 32, srow = lane >> 2, scol = 4 * (lane & 3);   // rows srow + 8 i
         float f;   // factor of the query's scores
         {
             // half a query into TMEM
-            float4 v[HC / 4];
-            const float4 *src = reinterpret_cast<const float4 *>(a.q + (size_t)(rq.row0 + (q < nq ? q / G : 0)) * a.ldq +
-                                                                 (size_t)(kvh * G + q % G) * HD + half * HC);
-            float mx = 0.0f;
+            const float4 *src[4];
 #pragma unroll
-            for (int i = 0; i < HC / 4; i++) v[i] = src[i];
+            for (int i = 0; i < 4; i++) {
+                const int qi = min(q0 + wrow + srow + 8 * i, nq - 1), t = qi / G;
+                src[i] = reinterpret_cast<const float4 *>(a.q + (size_t)(rq.row0 + t) * a.ldq +
+                                                          (size_t)(kvh * G + qi - t * G) * HD + half * HC + scol);
+            }
+            float4 v[4][HC / 16];
 #pragma unroll
-            for (int i = 0; i < HC / 4; i++)
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
-            red[1][half][row].x = mx;
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int c = 0; c < HC / 16; c++) v[i][c] = src[i][4 * c];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float mx = 0.0f;
+#pragma unroll
+                for (int c = 0; c < HC / 16; c++)
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i][c].x), fabsf(v[i][c].y)), fmaxf(fabsf(v[i][c].z), fabsf(v[i][c].w))));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                if ((lane & 3) == 0) red[1][half][wrow + srow + 8 * i].x = mx;
+            }
             mn_group_sync();
-            mx = fmaxf(mx, red[1][half ^ 1][row].x);
+            const float mx = fmaxf(red[1][0][row].x, red[1][1][row].x);
             // the row's largest element into [2^13, 2^14); a negative scale goes into the queries, since
             // the maxima are taken before the factor is applied
             const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
@@ -273,13 +308,17 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             f = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 13) << 23);
 #pragma unroll
             for (int c = 0; c < HC / 16; c++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) *reinterpret_cast<float4 *>(st + (srow + 8 * i) * 20 + scol) = v[i][c];
+                __syncwarp();
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 x = v[4 * c + i];
+                    const float4 x = *reinterpret_cast<const float4 *>(st + lane * 20 + 4 * i);
                     hi[2 * i] = split_h2(x.x * up, x.y * up, lo[2 * i]);
                     hi[2 * i + 1] = split_h2(x.z * up, x.w * up, lo[2 * i + 1]);
                 }
+                __syncwarp();
                 tmem_st8(t_q + tl + half * (HC / 2) + 8 * c, hi);
                 tmem_st8(t_q + tl + 64 + half * (HC / 2) + 8 * c, lo);
             }
@@ -303,7 +342,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             tmem_wait_ld();
             tmem_pin<HC>(v);
 #pragma unroll
-            for (int d = 0; d < HC; d++) acc[d] += __uint_as_float(v[d]);
+            for (int d = 0; d < HC; d += 2)
+                unf2(add2(f2(acc[d], acc[d + 1]), f2(__uint_as_float(v[d]), __uint_as_float(v[d + 1]))), acc[d], acc[d + 1]);
             tc_fence_before();
             mbar_arrive(oempty);
             return true;
@@ -319,13 +359,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             __syncwarp();
             tc_fence_after();
             uint32_t v[64];
+            float mx = -INFINITY, mxv = -INFINITY, shrink = 1.0f;
             tmem_ld32(t_s, v);
             tmem_ld32(t_s + 32, v + 32);
             const int t0 = p0 + 128 * j + 64 * half;
             const float4 ks = *reinterpret_cast<const float4 *>(&page_ks[e][4 * half]);
-            const float4 vs = *reinterpret_cast<const float4 *>(&page_vs[e][4 * half]);
             const float4 lv = *reinterpret_cast<const float4 *>(&page_lv[e][4 * half]);
-            const float fk[4] = {f * ks.x, f * ks.y, f * ks.z, f * ks.w};
+            const float fk[4] = {mn_factor(f * ks.x), mn_factor(f * ks.y), mn_factor(f * ks.z), mn_factor(f * ks.w)};
             // bit c: group c of 16 tokens lies in a block outside the cache
             const uint32_t bad = __ballot_sync(0xffffffffu, lane < 4 && page_at[e][4 * half + (lane & 3)] == -2);
             const bool whole = __all_sync(0xffffffffu, lim >= t0 + 63) && bad == 0;
@@ -340,7 +380,6 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     for (int k = 0; k < 16; k++) v[16 * c + k] = (mk >> k) & 1u ? v[16 * c + k] : 0xFF800000u;   // -inf
                 }
             }
-            float mx = -INFINITY, mxv = -INFINITY;
             {
                 const float lvc[4] = {lv.x, lv.y, lv.z, lv.w};
                 float x[4];
@@ -349,8 +388,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     x[c] = __uint_as_float(v[16 * c]);
 #pragma unroll
                     for (int k = 1; k < 16; k++) x[c] = fmaxf(x[c], __uint_as_float(v[16 * c + k]));
-                    // (no visible token: -inf, also where the scale is 0)
-                    x[c] = x[c] == -INFINITY ? x[c] : x[c] * fk[c];
+                    x[c] *= fk[c];
                     mx = fmaxf(mx, x[c]);
                     mxv = fmaxf(mxv, x[c] + lvc[c]);
                 }
@@ -367,30 +405,29 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 l *= ex2(m - mx);   // 0 at first
                 m = mx;
             }
-            float shrink = 1.0f;
             if (mxv > mv + KV8_LAG || (mv == -INFINITY && mxv > mv)) {
                 shrink = ex2(mv - mxv);
                 mv = mxv;
             }
             const float mref = m == -INFINITY ? 0.0f : m;
             const float cv = ex2(fminf(mref - mv + KV8_HEAD, 120.0f));
+            const float4 vs = *reinterpret_cast<const float4 *>(&page_vs[e][4 * half]);
+            // (read again: registers are what is short here)
+            const float4 ks2 = *reinterpret_cast<const float4 *>(&page_ks[e][4 * half]);
+            const float fk2[4] = {mn_factor(f * ks2.x), mn_factor(f * ks2.y), mn_factor(f * ks2.z), mn_factor(f * ks2.w)};
             const float cw[4] = {vs.x * cv, vs.y * cv, vs.z * cv, vs.w * cv};
-            const uint64_t nm = f2(-mref, -mref);
+            const uint64_t nm = f2(-mref, -mref), minus = f2(-1.0f, -1.0f);
             uint64_t sum = f2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const uint64_t fk2 = f2(fk[c], fk[c]), cw2 = f2(cw[c], cw[c]);
+                const uint64_t fkc = f2(fk2[c], fk2[c]), cw2 = f2(cw[c], cw[c]);
                 uint32_t w[16];
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
                     float x, y;
-                    unf2(fma2(f2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])), fk2, nm), x, y);
+                    unf2(fma2(f2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])), fkc, nm), x, y);
                     x = ex2(x);
                     y = ex2(y);
-                    if (!whole) {   // -inf times a scale of 0
-                        x = v[16 * c + k] == 0xFF800000u ? 0.0f : x;
-                        y = v[16 * c + k + 1] == 0xFF800000u ? 0.0f : y;
-                    }
                     const uint64_t p = f2(x, y);
                     sum = add2(sum, p);
                     float wx, wy;
@@ -398,7 +435,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     unf2(wt, wx, wy);
                     const __half2 h = __floats2half2_rn(wx, wy);
                     const float2 hf = __half22float2(h);
-                    unf2(add2(wt, f2(-hf.x, -hf.y)), wx, wy);
+                    unf2(fma2(f2(hf.x, hf.y), minus, wt), wx, wy);
                     const __half2 lo = __floats2half2_rn(wx, wy);
                     w[k / 2] = *reinterpret_cast<const uint32_t *>(&h);
                     w[8 + k / 2] = *reinterpret_cast<const uint32_t *>(&lo);
@@ -422,31 +459,37 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         }
         if (ok && nt > 0) drain(nt - 1);
-        // The last P V product is done, so no product reads shared memory any more (after an abort one
-        // may, but then nothing is written).  Outputs in units of 2^m, through shared memory.
-        float *so = reinterpret_cast<float *>(sm + M::K);     // [HD][129]
-        float2 *st = reinterpret_cast<float2 *>(so + HD * 129);   // [2][128]: m, l of a query's halves
-        mn_group_sync();
-        st[128 * half + row] = make_float2(m, l);
-        mn_group_sync();
-        {
-            const float L = st[row].y + st[128 + row].y;
+        // outputs in units of 2^m
+        red[0][half][row].x = l;
+        ok = bar_and(1, 256, ok);
+        if (ok) {
+            const float L = l + red[0][half ^ 1][row].x;
             const float inv = ns > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
-            const float back = mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f));
+            const float back = (mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f))) * inv;
+            float *dst[4];
 #pragma unroll
-            for (int d = 0; d < HC; d++) so[(half * HC + d) * 129 + row] = acc[d] * back * inv;
-        }
-        mn_group_sync();
-        if (!*abortp) {
-            // a warp per query, lanes over the head dim
-            for (int i = warp - MN_LOADERS / 32; i < 128 && q0 + i < nq; i += 8) {
-                const int oq = q0 + i, orow = rq.row0 + oq / G, h = kvh * G + oq % G;
-                float *rec = a.part + (((size_t)orow * a.H + h) * a.S + split) * (HD + 4);
-                float *dst = ns > 1 ? rec + 4 : a.out + (size_t)orow * a.ldo + (size_t)h * HD;
+            for (int i = 0; i < 4; i++) {
+                const int qi = q0 + wrow + srow + 8 * i, t = qi / G, h = kvh * G + qi - t * G;
+                float *to = ns > 1 ? a.part + (((size_t)(rq.row0 + t) * a.H + h) * a.S + split) * (HD + 4) + 4
+                                   : a.out + (size_t)(rq.row0 + t) * a.ldo + (size_t)h * HD;
+                dst[i] = qi < nq ? to + half * HC + scol : nullptr;
+                // m and L of the rows, handed to the lanes that know their records
+                const float mi = __shfl_sync(0xffffffffu, m, srow + 8 * i), Li = __shfl_sync(0xffffffffu, L, srow + 8 * i);
+                if (ns > 1 && half == 0 && scol == 0 && dst[i]) *reinterpret_cast<float2 *>(to - 4) = make_float2(mi, Li);
+            }
 #pragma unroll
-                for (int d = lane; d < HD; d += 32) dst[d] = so[d * 129 + i];
-                if (ns > 1 && lane == 0)
-                    *reinterpret_cast<float2 *>(rec) = make_float2(st[i].x, st[i].y + st[128 + i].y);
+            for (int c = 0; c < HC / 16; c++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(st + lane * 20 + 4 * i) =
+                        make_float4(acc[16 * c + 4 * i] * back, acc[16 * c + 4 * i + 1] * back, acc[16 * c + 4 * i + 2] * back,
+                                    acc[16 * c + 4 * i + 3] * back);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (dst[i])
+                        *reinterpret_cast<float4 *>(dst[i] + 16 * c) = *reinterpret_cast<const float4 *>(st + (srow + 8 * i) * 20 + scol);
+                __syncwarp();
             }
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -465,10 +508,11 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 if (ok && j >= 2) ok = mn_wait(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t kb = smb + M::K + s * M::TILE, d = tmem + 128 * s;
+                const uint64_t kd = sdesc(smb + M::K + s * M::TILE, MN_CHUNK, 128);
+                const uint32_t d = tmem + 128 * s;
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
-                    const uint64_t bd = sdesc(kb + k * 2 * MN_CHUNK, MN_CHUNK, 128);
+                    const uint64_t bd = kd + (uint64_t)((k * 2 * MN_CHUNK) >> 4);
                     mma_f16_ts(d, t_q + 8 * k, bd, idesc, k != 0);
                     mma_f16_ts(d, t_q + 64 + 8 * k, bd, idesc, 1u);
                 }
@@ -486,26 +530,27 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 if (ok && j >= 1) ok = mn_wait(oempty, (j - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t vb = smb + M::V + s * M::TILE, p = tmem + 128 * s;
+                const uint64_t vd = sdesc(smb + M::V + s * M::TILE, 128, MN_CHUNK);
+                const uint32_t p = tmem + 128 * s;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const uint64_t bd = sdesc(vb + k * 256, 128, MN_CHUNK);
+                    const uint64_t bd = vd + (uint64_t)((k * 256) >> 4);
                     mma_f16_ts(t_o, p + 16 * k, bd, idesc, k != 0);
                     mma_f16_ts(t_o, p + 16 * k + 8, bd, idesc, 1u);
                 }
                 mma_commit(ofull(s));
             }
-        } else if (warp == 18 && lane < 8) {
+        } else if (warp == 18) {
             // ------------------------------ blocks and scales ------------------------------
-            const int *trow = rq.table;
-            for (int j = 0; j < nt; j++) {
-                const int e = j % MN_PAGES;
-                if (j >= MN_PAGES && !mn_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI)) break;
-                const int p = p0 + 128 * j + 16 * lane;
+            // lane = (tile of four, group of 16 tokens)
+            bool ok = true;
+#pragma unroll 1
+            for (int t = 0; t < nt && ok; t += 4) {
+                const int p = p0 + 128 * t + 16 * lane;
                 long long at = -1;
                 float ks = 0.0f, vs = 0.0f;
-                if (p < rq.kvlen) {
-                    const int blk = trow[p / bs];
+                if (p < rq.kvlen && t + (lane >> 3) < nt) {
+                    const int blk = rq.table[p / bs];
                     if (blk >= 0 && blk < a.kv.n_blocks) {
                         const size_t bh = (size_t)blk * KH + kvh;
                         at = (long long)((bh * bs + p % bs) * HD);
@@ -516,11 +561,20 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                         vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
                     }
                 }
-                page_at[e][lane] = at;
-                page_ks[e][lane] = ks;
-                page_vs[e][lane] = vs;
-                page_lv[e][lane] = lg2(vs);
-                mbar_arrive(gfull(e));
+                const float lv = lg2(vs);
+                for (int k = 0; k < 4 && t + k < nt; k++) {
+                    const int j = t + k, e = j % MN_PAGES;
+                    if (j >= MN_PAGES) ok = mn_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane >> 3 == k) {
+                        page_at[e][lane & 7] = at;
+                        page_ks[e][lane & 7] = ks;
+                        page_vs[e][lane & 7] = vs;
+                        page_lv[e][lane & 7] = lv;
+                        mbar_arrive(gfull(e));
+                    }
+                }
             }
         }
         __syncwarp();
