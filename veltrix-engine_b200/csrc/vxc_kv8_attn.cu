@@ -513,7 +513,7 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
 
 // How a call is cut: kernel, queries per CTA and splits.
 struct AttnPlan {
-    int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), KV8_TILE_Q (k_kv8_attn_many)
+    int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), 32, 64 or 128 (k_kv8_attn_many)
     int tiles;     // k_kv8_attn_many: tiles of all requests at most
     int S, sl_min;
     int pages;     // blocks a split may touch (k_kv8_attn_few)
@@ -545,8 +545,8 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         if (S > 8 && tokens <= 8 * 512) S = 8;
         if (S < even) S = even;
     } else {
-        p.nq = KV8_TILE_Q;
-        const long long full = (long long)n_rows * G / KV8_TILE_Q;
+        p.nq = most <= 32 ? 32 : most <= 64 ? 64 : 128;
+        const long long full = (long long)n_rows * G / p.nq;
         p.tiles = (int)(full + n_req);
         p.sl_min = 512;
         const long long busy = n_req < n_rows ? n_req : n_rows;
@@ -557,7 +557,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
     if (S > need) S = need;
     // k_kv8_attn_few: a tensor core's sums lose up to an ulp per step: 8192 tokens are 128 steps per
     // warp, 5e-6 at most
-    const long long least = p.nq < KV8_TILE_Q ? (tokens + 8191) / 8192 : 1;
+    const long long least = p.nq <= ATTN_FEW_MAX ? (tokens + 8191) / 8192 : 1;
     if (S > 64) S = 64;
     if (S < least) S = least;
     p.S = (int)(S < 1 ? 1 : S);
@@ -568,7 +568,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
 }
 
 // Whether the splits leave records for k_kv8_attn_join.
-static bool attn_records(const AttnPlan &p) { return p.S > (p.nq == KV8_TILE_Q ? 1 : 8); }
+static bool attn_records(const AttnPlan &p) { return p.S > (p.nq > ATTN_FEW_MAX ? 1 : 8); }
 
 extern "C" size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new,
                                                int max_blocks) {
@@ -607,8 +607,8 @@ static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st)
     a.err = vxc_device_error_ptr();
     const vxc_kv8 *kv = &a.kv;
     const int hd = kv->head_dim;
-    if (p.nq == KV8_TILE_Q) {
-        VXC_CUDA_OK(kv8_attn_many(a, p.tiles, st));
+    if (p.nq > ATTN_FEW_MAX) {
+        VXC_CUDA_OK(kv8_attn_many(a, p.nq, p.tiles, st));
     } else {
         attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);
         size_t smem = (size_t)4 * FEW_STAGES * (hd * 64) + (size_t)p.pages * (sizeof(int) + sizeof(float4));

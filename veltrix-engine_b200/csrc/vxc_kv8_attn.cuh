@@ -92,11 +92,12 @@ struct Kv8Req {
     bool over;       // something was clamped
 };
 __device__ __forceinline__ int kv8_row0(const Kv8AttnArgs &a, int r) { return a.row0 ? a.row0[r] : r * a.max_new; }
-__device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
+// table row s (none if negative), first row r0, end r1, position pos
+__device__ __forceinline__ Kv8Req kv8_req_of(const Kv8AttnArgs &a, int s, int r0, int r1, int pos) {
     Kv8Req q;
-    const int r0 = kv8_row0(a, r), s = a.seq ? a.seq[r] : r, r1 = s < 0 ? r0 : kv8_row0(a, r + 1);
+    if (s < 0) r1 = r0;
     q.table = a.table + (size_t)max(s, 0) * a.max_blocks;
-    q.pos = a.pos[r];
+    q.pos = pos;
     q.row0 = max(r0, 0);
     long long T = (long long)r1 - r0;
     const long long cap = (long long)a.max_blocks * a.kv.block_size;
@@ -107,6 +108,9 @@ __device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
     q.kvlen = q.T > 0 ? max(q.pos + q.T, 0) : 0;
     return q;
 }
+__device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
+    return kv8_req_of(a, a.seq ? a.seq[r] : r, kv8_row0(a, r), kv8_row0(a, r + 1), a.pos[r]);
+}
 
 // Splits of a request: enough for SL_min tokens each, at most S.
 __device__ __forceinline__ int kv8_splits(int kvlen, int sl_min, int S, int &SL) {
@@ -116,6 +120,5 @@ __device__ __forceinline__ int kv8_splits(int kvlen, int sl_min, int S, int &SL)
 }
 
 // Many queries per kv head (vxc_kv8_attn_many.cu): launch over at most `tiles`
-// tiles of KV8_TILE_Q queries.
-#define KV8_TILE_Q 128
-cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tiles, cudaStream_t st);
+// tiles of tile_q (32, 64 or 128) queries.
+cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tile_q, int tiles, cudaStream_t st);

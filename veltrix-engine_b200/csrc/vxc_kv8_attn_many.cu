@@ -60,8 +60,9 @@ template <int HD>
 struct MnSmem {
     static constexpr int TILE = HD / 8 * MN_CHUNK;          // one fp16 tile of 128 rows
     static constexpr int PIECE = 128 * (HD == 96 ? 128 : HD);   // raw bytes of one (96: as 8 units per row)
-    static constexpr int STAGED = 32 * 20 * 4;                  // a softmax warp's 32 rows x 16 columns, 20 floats a row
-    static constexpr int K = 0, V = 2 * TILE, RAW = 4 * TILE, OUT = RAW + MN_AHEAD * PIECE, BYTES = OUT + 8 * STAGED;
+    // V's tiles, before them the queries and after them the outputs: 128 rows of HD + 4 floats
+    static constexpr int QO = 128 * (HD + 4) * 4, VQO = 2 * TILE > QO ? 2 * TILE : QO;
+    static constexpr int K = 0, RAW = 2 * TILE, V = RAW + MN_AHEAD * PIECE, BYTES = V + VQO;
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
@@ -123,7 +124,7 @@ __device__ __forceinline__ void mn_group_sync() { asm volatile("bar.sync 1, 256;
 // softmax warp has not got yet, and that warp would wait for them for ever.
 __device__ __forceinline__ void mn_roles_done() { asm volatile("bar.sync 2, %0;" ::"n"(MN_THREADS) : "memory"); }
 
-template <int TYPE, int HD>
+template <int TYPE, int HD, int TQ>
 __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnArgs a) {
     using M = MnSmem<HD>;
     extern __shared__ __align__(128) unsigned char sm[];
@@ -133,37 +134,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     __shared__ float2 red[2][2][128];              // [tile parity][half][query]: maxima of half a tile
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ struct {
+        const int *table;
+        int q0, nq, row0, pos, kvlen, ns, SL;   // nq 0: no work
+    } item;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
-    pdl_trigger();
-    pdl_wait();
-
-    // request and query tile: tiles of request r begin at floor(row0 G / 128) + r, which leaves
-    // every request as many as it needs; later tiles (longer contexts) first
-    const int idx = (int)gridDim.x - 1 - (int)blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-    int r = 0;
-    for (int len = a.n_req; len > 1;) {   // 32 places a step
-        const int step = (len + 31) / 32, at = lane * step;
-        const bool le = at < len && (long long)max(kv8_row0(a, r + at), 0) * G / KV8_TILE_Q + r + at <= idx;
-        const unsigned mask = __ballot_sync(0xffffffffu, le);
-        const int k = mask ? 31 - __clz(mask) : 0;
-        r += k * step;
-        len = min(step, len - k * step);
-    }
-    const Kv8Req rq = kv8_req(a, r);
-    const long long tile0 = (long long)rq.row0 * G / KV8_TILE_Q + r;
-    if (kvh == 0 && split == 0 && tid == 0 && ((rq.over && idx == tile0) || (idx == 0 && kv8_row0(a, a.n_req) > a.n_rows)))
-        vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
-    const int nq = rq.T * G;
-    const long long q0l = (idx - tile0) * KV8_TILE_Q;
-    if (q0l < 0 || q0l >= nq) return;
-    const int q0 = (int)q0l;
-    int SL;
-    const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
-    if (split >= ns) return;
-    const int p0 = split * SL, p1 = min(p0 + SL, rq.pos + (min(q0 + KV8_TILE_Q, nq) - 1) / G + 1);
-    const int nt = p1 > p0 ? (p1 - p0 + 127) >> 7 : 0;
-
+    const int kvh = blockIdx.y, split = blockIdx.z;
     const uint32_t bar0 = smem_u32(bars);
     auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (loaders)
     auto vfull = [&](int s) { return bar0 + 8u * (2 + s); };
@@ -173,7 +150,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     const uint32_t oempty = bar0 + 8u * 14, qfull = bar0 + 8u * 15;   // O read; queries stored (256 threads)
     auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks and scales of a tile (8 lanes)
     auto gempty = [&](int s) { return bar0 + 8u * (26 + s); };     // loaders (after V) and the softmax group are done with them
-    if (tid == 0) {
+    pdl_trigger();
+    if (tid == 32) {
         for (int s = 0; s < 2; s++) {
             mbar_init(kfull(s), MN_LOADERS), mbar_init(vfull(s), MN_LOADERS);
             mbar_init(sfull(s), 1), mbar_init(pfull(s), 256), mbar_init(ofull(s), 1);
@@ -185,9 +163,60 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         mbar_init_fence();
     }
     if (warp == 16) tmem_alloc(smem_u32(&tmem_slot), 512u);
+    pdl_wait();
+    if (warp == 0) {
+        // request and query tile: tiles of request r begin at floor(row0 G / TQ) + r, which leaves
+        // every request as many as it needs; later tiles (longer contexts) first.  (One warp: the
+        // same work by all of them took 2000 cycles more.)
+        const int idx = (int)gridDim.x - 1 - (int)blockIdx.x;
+        int r = 0, len = a.n_req, r0, r1, pos, seq;
+        do {   // 32 places a step
+            const int step = (len + 31) / 32, at = lane * step, ri = r + at;
+            const bool in = at < len;
+            r0 = in ? kv8_row0(a, ri) : 0;
+            if (step == 1) {
+                r1 = in ? kv8_row0(a, ri + 1) : 0;
+                pos = in ? a.pos[ri] : 0;
+                seq = in && a.seq ? a.seq[ri] : ri;
+            }
+            const bool le = in && (long long)max(r0, 0) * G / TQ + ri <= idx;
+            const unsigned mask = __ballot_sync(0xffffffffu, le);
+            const int k = mask ? 31 - __clz(mask) : 0;
+            r += k * step;
+            if (step == 1) {
+                r0 = __shfl_sync(0xffffffffu, r0, k);
+                r1 = __shfl_sync(0xffffffffu, r1, k);
+                pos = __shfl_sync(0xffffffffu, pos, k);
+                seq = __shfl_sync(0xffffffffu, seq, k);
+                break;
+            }
+            len = min(step, len - k * step);
+        } while (true);
+        const Kv8Req rq = kv8_req_of(a, seq, r0, r1, pos);
+        const long long tile0 = (long long)rq.row0 * G / TQ + r;
+        if (kvh == 0 && split == 0 && lane == 0 &&
+            ((rq.over && idx == tile0) || (idx == 0 && kv8_row0(a, a.n_req) > a.n_rows)))
+            vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+        const int nq = rq.T * G;
+        const long long q0 = (idx - tile0) * TQ;
+        int SL;
+        const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
+        if (lane == 0) {
+            const bool work = q0 >= 0 && q0 < nq && split < ns;
+            item.q0 = (int)q0, item.nq = work ? nq : 0, item.row0 = rq.row0, item.pos = rq.pos, item.kvlen = rq.kvlen;
+            item.ns = ns, item.SL = SL, item.table = rq.table;
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const int q0 = item.q0, nq = item.nq, row0 = item.row0, pos = item.pos, kvlen = item.kvlen, ns = item.ns;
+    const int p0 = split * item.SL, p1 = min(p0 + item.SL, pos + (min(q0 + TQ, nq) - 1) / G + 1);
+    const int nt = p1 > p0 ? (p1 - p0 + 127) >> 7 : 0;
+    if (nq == 0) {   // nothing here
+        if (warp == 16) tmem_dealloc(tmem_slot, 512u);
+        return;
+    }
     const uint32_t tmem = tmem_slot, t_o = tmem + 256, t_q = tmem + 384;   // Q: hi in HD / 2 columns, lo 64 columns on
     volatile int *abortp = &abort_flag;
     unsigned int *err = a.err;
@@ -213,7 +242,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 const uint8_t *base = (const uint8_t *)(isv ? a.kv.v : a.kv.k);
                 const uint8_t *src = base + (tr & 15) * HD + c * 16;
                 const uint32_t dst = raw + (i % MN_AHEAD) * M::PIECE;
-                const int live = rq.kvlen - (p0 + 128 * j);
+                const int live = kvlen - (p0 + 128 * j);
                 if (on) {
 #pragma unroll
                     for (int k = 0; k < NP; k++) {
@@ -235,6 +264,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             const bool isv = is_v(i);
             cp_wait<MN_AHEAD - 1>();
             if (j >= 2) ok = mn_wait(isv ? ofull(s) : sfull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            if (isv && j == 0) ok = mn_wait(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);   // V's space held the queries
             if (!ok) break;
             unsigned char *dst = sm + (isv ? M::V : M::K) + s * M::TILE + 2 * c * MN_CHUNK + tr * 16;
             const unsigned char *src = sm + M::RAW + tid * 16 + (i % MN_AHEAD) * M::PIECE;
@@ -267,40 +297,49 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         // ------------------------------ softmax ------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         constexpr int HC = HD / 2;   // elements of a query, columns of O per thread
-        const int half = (warp >> 2) - MN_LOADERS / 128, row = tid & 127;
+        // TQ < 128: the tile's queries stand in 128 / TQ parts of its rows, and each part weighs its own
+        // tokens of a tile (the others' weights are 0 there): NG groups of 16 tokens per thread
+        constexpr int NP = 128 / TQ, NG = 4 / NP;
+        const int half = (warp >> 2) - MN_LOADERS / 128, row = tid & 127, part = row / TQ, qrow = row % TQ;
         const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
-        const int q = q0 + row;
-        // Global rows are read and written 16 columns at a time, 4 lanes a row (a lane per row would touch
-        // 32 lines an instruction), and change hands in the warp's own space: lane = row there.
-        float *st = reinterpret_cast<float *>(sm + M::OUT + (warp - MN_LOADERS / 32) * M::STAGED);
-        const int wrow = (warp & 3) * 32, srow = lane >> 2, scol = 4 * (lane & 3);   // rows srow + 8 i
+        const int q = q0 + qrow;
+        // Global rows are read and written whole, LPR lanes a row (a lane per row would touch 32 lines an
+        // instruction), and change hands in shared memory
+        constexpr int LPR = HD == 96 ? 32 : HD / 4, RPW = 32 / LPR, XS = HD + 4;
+        constexpr int RPS = 8 * RPW;   // rows a step
+        const int srow = (warp - MN_LOADERS / 32) * RPW + lane / LPR, scol = 4 * (lane % LPR);   // rows srow + RPS i
+        const bool son = scol < HD;
+        // query srow's row and head, and how far RPS queries are
+        const int t_at = (q0 + srow) / G, g_at = q0 + srow - t_at * G, t_by = RPS / G, g_by = RPS - t_by * G;
+        float *xs = reinterpret_cast<float *>(sm + M::V);
         float f;   // factor of the query's scores
         {
             // half a query into TMEM
-            const float4 *src[4];
+            int g = g_at;
+            const float *src = a.q + (size_t)(row0 + t_at) * a.ldq + (size_t)(kvh * G + g) * HD + scol;
+            const long long step = (long long)t_by * a.ldq + (long long)g_by * HD, wrap = a.ldq - (long long)G * HD;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int qi = min(q0 + wrow + srow + 8 * i, nq - 1), t = qi / G;
-                src[i] = reinterpret_cast<const float4 *>(a.q + (size_t)(rq.row0 + t) * a.ldq +
-                                                          (size_t)(kvh * G + qi - t * G) * HD + half * HC + scol);
+            for (int i = 0; i < TQ / RPS; i++) {
+                const int rw = srow + RPS * i;
+                const bool have = rw < nq - q0;
+                if (son) cp_async_zfill<16>(smem_u32(xs + rw * XS + scol), have ? src : a.q, have);
+                src += step;
+                g += g_by;
+                if (g >= G) g -= G, src += wrap;
             }
-            float4 v[4][HC / 16];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int c = 0; c < HC / 16; c++) v[i][c] = src[i][4 * c];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float mx = 0.0f;
-#pragma unroll
-                for (int c = 0; c < HC / 16; c++)
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i][c].x), fabsf(v[i][c].y)), fmaxf(fabsf(v[i][c].z), fabsf(v[i][c].w))));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if ((lane & 3) == 0) red[1][half][wrow + srow + 8 * i].x = mx;
-            }
+            cp_commit();
+            cp_wait<0>();
             mn_group_sync();
-            const float mx = fmaxf(red[1][0][row].x, red[1][1][row].x);
+            float4 v[HC / 4];
+            float mx = 0.0f;
+#pragma unroll
+            for (int c = 0; c < HC / 4; c++) {
+                v[c] = *reinterpret_cast<const float4 *>(xs + qrow * XS + half * HC + 4 * c);
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
+            }
+            red[1][half][row].x = mx;
+            mn_group_sync();
+            mx = fmaxf(mx, red[1][half ^ 1][row].x);
             // the row's largest element into [2^13, 2^14); a negative scale goes into the queries, since
             // the maxima are taken before the factor is applied
             const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
@@ -308,17 +347,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             f = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 13) << 23);
 #pragma unroll
             for (int c = 0; c < HC / 16; c++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) *reinterpret_cast<float4 *>(st + (srow + 8 * i) * 20 + scol) = v[i][c];
-                __syncwarp();
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(st + lane * 20 + 4 * i);
+                    const float4 x = v[4 * c + i];
                     hi[2 * i] = split_h2(x.x * up, x.y * up, lo[2 * i]);
                     hi[2 * i + 1] = split_h2(x.z * up, x.w * up, lo[2 * i + 1]);
                 }
-                __syncwarp();
                 tmem_st8(t_q + tl + half * (HC / 2) + 8 * c, hi);
                 tmem_st8(t_q + tl + 64 + half * (HC / 2) + 8 * c, lo);
             }
@@ -330,7 +365,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         float acc[HC];
 #pragma unroll
         for (int d = 0; d < HC; d++) acc[d] = 0.0f;
-        const int lim = q < nq ? rq.pos + q / G : -1;
+        const int lim = q < nq ? pos + q / G : -1;
         // adds O of tile j to the registers
         auto drain = [&](int j) -> bool {
             const bool ok = mn_wait(ofull(j & 1), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
@@ -352,52 +387,54 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
 #pragma unroll 1
         for (int j = 0; j < nt; j++) {
             const int e = j % MN_PAGES, b = j & 1;
-            const uint32_t t_s = tmem + tl + 128 * b + 64 * half;
+            const uint32_t t_s = tmem + tl + 128 * b + 64 * half, t_g = t_s + 16 * NG * part;
+            const int g0 = 4 * half + NG * part;   // the thread's first group of 16 tokens
             // (S is there, so the loaders have seen the tile's blocks and scales, and so does this thread)
             ok = ok && mn_wait(sfull(b), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
             // (after a failed wait the scores are garbage; every warp leaves at the barrier below)
             __syncwarp();
             tc_fence_after();
-            uint32_t v[64];
+            uint32_t v[16 * NG];
             float mx = -INFINITY, mxv = -INFINITY, shrink = 1.0f;
-            tmem_ld32(t_s, v);
-            tmem_ld32(t_s + 32, v + 32);
-            const int t0 = p0 + 128 * j + 64 * half;
-            const float4 ks = *reinterpret_cast<const float4 *>(&page_ks[e][4 * half]);
-            const float4 lv = *reinterpret_cast<const float4 *>(&page_lv[e][4 * half]);
-            const float fk[4] = {mn_factor(f * ks.x), mn_factor(f * ks.y), mn_factor(f * ks.z), mn_factor(f * ks.w)};
+            if (NG == 1) {
+                tmem_ld16(t_g, v);
+            } else {
+                tmem_ld32(t_g, v);
+                if (NG == 4) tmem_ld32(t_g + 32, v + 16 * (NG - 2));
+            }
+            const int t0 = p0 + 128 * j + 16 * g0;
+            float fk[NG];
+#pragma unroll
+            for (int c = 0; c < NG; c++) fk[c] = mn_factor(f * page_ks[e][g0 + c]);
             // bit c: group c of 16 tokens lies in a block outside the cache
-            const uint32_t bad = __ballot_sync(0xffffffffu, lane < 4 && page_at[e][4 * half + (lane & 3)] == -2);
-            const bool whole = __all_sync(0xffffffffu, lim >= t0 + 63) && bad == 0;
+            const uint32_t bad = __ballot_sync(0xffffffffu, lane < NG && page_at[e][g0 + (lane & (NG - 1))] == -2);
+            const bool whole = __all_sync(0xffffffffu, lim >= t0 + 16 * NG - 1) && bad == 0;
             tmem_wait_ld();
-            tmem_pin<64>(v);
+            tmem_pin<16 * NG>(v);
             if (!whole) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {   // visible tokens of group c: the low bits of a mask
+                for (int c = 0; c < NG; c++) {   // visible tokens of group c: the low bits of a mask
                     const int n = lim - (t0 + 16 * c) + 1;
                     const uint32_t mk = ((bad >> c) & 1u) || n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
 #pragma unroll
                     for (int k = 0; k < 16; k++) v[16 * c + k] = (mk >> k) & 1u ? v[16 * c + k] : 0xFF800000u;   // -inf
                 }
             }
-            {
-                const float lvc[4] = {lv.x, lv.y, lv.z, lv.w};
-                float x[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    x[c] = __uint_as_float(v[16 * c]);
+            for (int c = 0; c < NG; c++) {
+                float x = __uint_as_float(v[16 * c]);
 #pragma unroll
-                    for (int k = 1; k < 16; k++) x[c] = fmaxf(x[c], __uint_as_float(v[16 * c + k]));
-                    x[c] *= fk[c];
-                    mx = fmaxf(mx, x[c]);
-                    mxv = fmaxf(mxv, x[c] + lvc[c]);
-                }
+                for (int k = 1; k < 16; k++) x = fmaxf(x, __uint_as_float(v[16 * c + k]));
+                x *= fk[c];
+                mx = fmaxf(mx, x);
+                mxv = fmaxf(mxv, x + page_lv[e][g0 + c]);
             }
             red[b][half][row] = make_float2(mx, mxv);
             ok = bar_and(1, 256, ok);   // the softmax warps go on together or not at all
             if (!ok) break;
-            {
-                const float2 o = red[b][half ^ 1][row];
+#pragma unroll
+            for (int i = 1; i < 2 * NP; i++) {   // the query's other threads
+                const float2 o = red[b][half ^ (i & 1)][qrow + TQ * ((part + (i >> 1)) % NP)];
                 mx = fmaxf(mx, o.x);
                 mxv = fmaxf(mxv, o.y);
             }
@@ -411,16 +448,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
             const float mref = m == -INFINITY ? 0.0f : m;
             const float cv = ex2(fminf(mref - mv + KV8_HEAD, 120.0f));
-            const float4 vs = *reinterpret_cast<const float4 *>(&page_vs[e][4 * half]);
-            // (read again: registers are what is short here)
-            const float4 ks2 = *reinterpret_cast<const float4 *>(&page_ks[e][4 * half]);
-            const float fk2[4] = {mn_factor(f * ks2.x), mn_factor(f * ks2.y), mn_factor(f * ks2.z), mn_factor(f * ks2.w)};
-            const float cw[4] = {vs.x * cv, vs.y * cv, vs.z * cv, vs.w * cv};
             const uint64_t nm = f2(-mref, -mref), minus = f2(-1.0f, -1.0f);
             uint64_t sum = f2(0.0f, 0.0f);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint64_t fkc = f2(fk2[c], fk2[c]), cw2 = f2(cw[c], cw[c]);
+            for (int c = 0; c < NG; c++) {
+                // (read again: registers are what is short here)
+                const float fg = mn_factor(f * page_ks[e][g0 + c]), cw = page_vs[e][g0 + c] * cv;
+                const uint64_t fkc = f2(fg, fg), cw2 = f2(cw, cw);
                 uint32_t w[16];
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
@@ -441,7 +475,13 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                     w[8 + k / 2] = *reinterpret_cast<const uint32_t *>(&lo);
                 }
                 // hi in columns 0-7 of the group's 16, lo in 8-15
-                tmem_st16(t_s + 16 * c, w);
+                tmem_st16(t_g + 16 * c, w);
+            }
+            if (NP > 1) {
+                const uint32_t none[16] = {};
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    if (g / NG != part) tmem_st16(t_s + 16 * g, none);
             }
             {
                 float x, y;
@@ -463,33 +503,42 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         red[0][half][row].x = l;
         ok = bar_and(1, 256, ok);
         if (ok) {
-            const float L = l + red[0][half ^ 1][row].x;
+            float L = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; i++) L += red[0][0][qrow + TQ * i].x + red[0][1][qrow + TQ * i].x;
             const float inv = ns > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
             const float back = (mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f))) * inv;
-            float *dst[4];
+            // (every product has ended: V's space is free)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int qi = q0 + wrow + srow + 8 * i, t = qi / G, h = kvh * G + qi - t * G;
-                float *to = ns > 1 ? a.part + (((size_t)(rq.row0 + t) * a.H + h) * a.S + split) * (HD + 4) + 4
-                                   : a.out + (size_t)(rq.row0 + t) * a.ldo + (size_t)h * HD;
-                dst[i] = qi < nq ? to + half * HC + scol : nullptr;
-                // m and L of the rows, handed to the lanes that know their records
-                const float mi = __shfl_sync(0xffffffffu, m, srow + 8 * i), Li = __shfl_sync(0xffffffffu, L, srow + 8 * i);
-                if (ns > 1 && half == 0 && scol == 0 && dst[i]) *reinterpret_cast<float2 *>(to - 4) = make_float2(mi, Li);
+            for (int d = 0; d < HC; d += 4)
+                *reinterpret_cast<float4 *>(xs + row * XS + half * HC + d) =
+                    make_float4(acc[d] * back, acc[d + 1] * back, acc[d + 2] * back, acc[d + 3] * back);
+            if (ns > 1 && half == 0 && part == 0 && q < nq) {
+                const int t = q / G, h = kvh * G + q - t * G;
+                *reinterpret_cast<float2 *>(a.part + (((size_t)(row0 + t) * a.H + h) * a.S + split) * (HD + 4)) = make_float2(m, L);
             }
+            mn_group_sync();
+            int g = g_at;
+            const size_t hw = ns > 1 ? (size_t)a.S * (HD + 4) : HD;   // a head's floats, a row's
+            const long long ld = ns > 1 ? (long long)a.H * hw : a.ldo;
+            float *dst = (ns > 1 ? a.part + (size_t)split * (HD + 4) + 4 : a.out) + (size_t)(row0 + t_at) * ld +
+                         (size_t)(kvh * G + g) * hw + scol;
+            const long long step = t_by * ld + (long long)(g_by * hw), wrap = ld - (long long)(G * hw);
 #pragma unroll
-            for (int c = 0; c < HC / 16; c++) {
+            for (int i = 0; i < TQ / RPS; i++) {
+                const int rw = srow + RPS * i;
+                if (son && rw < nq - q0) {
+                    float4 x = *reinterpret_cast<const float4 *>(xs + rw * XS + scol);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(st + lane * 20 + 4 * i) =
-                        make_float4(acc[16 * c + 4 * i] * back, acc[16 * c + 4 * i + 1] * back, acc[16 * c + 4 * i + 2] * back,
-                                    acc[16 * c + 4 * i + 3] * back);
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (dst[i])
-                        *reinterpret_cast<float4 *>(dst[i] + 16 * c) = *reinterpret_cast<const float4 *>(st + (srow + 8 * i) * 20 + scol);
-                __syncwarp();
+                    for (int k = 1; k < NP; k++) {
+                        const float4 y = *reinterpret_cast<const float4 *>(xs + (rw + TQ * k) * XS + scol);
+                        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                    }
+                    *reinterpret_cast<float4 *>(dst) = x;
+                }
+                dst += step;
+                g += g_by;
+                if (g >= G) g -= G, dst += wrap;
             }
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -549,8 +598,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 const int p = p0 + 128 * t + 16 * lane;
                 long long at = -1;
                 float ks = 0.0f, vs = 0.0f;
-                if (p < rq.kvlen && t + (lane >> 3) < nt) {
-                    const int blk = rq.table[p / bs];
+                if (p < kvlen && t + (lane >> 3) < nt) {
+                    const int blk = item.table[p / bs];
                     if (blk >= 0 && blk < a.kv.n_blocks) {
                         const size_t bh = (size_t)blk * KH + kvh;
                         at = (long long)((bh * bs + p % bs) * HD);
@@ -597,15 +646,23 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     if (warp == 16) tmem_dealloc(tmem, 512u);
 }
 
+typedef void (*many_kernel_t)(const Kv8AttnArgs);
+template <int TYPE, int HD>
+static many_kernel_t many_kernel(int tile_q) {
+    return tile_q == 32   ? k_kv8_attn_many<TYPE, HD, 32>
+           : tile_q == 64 ? k_kv8_attn_many<TYPE, HD, 64>
+                          : k_kv8_attn_many<TYPE, HD, 128>;
+}
+
 template <int TYPE>
-static cudaError_t launch_many(const Kv8AttnArgs &a, int tiles, cudaStream_t st) {
-    void (*f)(const Kv8AttnArgs) = nullptr;
+static cudaError_t launch_many(const Kv8AttnArgs &a, int tile_q, int tiles, cudaStream_t st) {
+    many_kernel_t f = nullptr;
     size_t smem = 0;
     switch (a.kv.head_dim) {
-        case 32: f = k_kv8_attn_many<TYPE, 32>; smem = MnSmem<32>::BYTES; break;
-        case 64: f = k_kv8_attn_many<TYPE, 64>; smem = MnSmem<64>::BYTES; break;
-        case 96: f = k_kv8_attn_many<TYPE, 96>; smem = MnSmem<96>::BYTES; break;
-        default: f = k_kv8_attn_many<TYPE, 128>; smem = MnSmem<128>::BYTES; break;
+        case 32: f = many_kernel<TYPE, 32>(tile_q); smem = MnSmem<32>::BYTES; break;
+        case 64: f = many_kernel<TYPE, 64>(tile_q); smem = MnSmem<64>::BYTES; break;
+        case 96: f = many_kernel<TYPE, 96>(tile_q); smem = MnSmem<96>::BYTES; break;
+        default: f = many_kernel<TYPE, 128>(tile_q); smem = MnSmem<128>::BYTES; break;
     }
     // TMEM is allocated whole: one CTA per SM, so at least half of the shared memory is asked for
     if (smem < 116 * 1024) smem = 116 * 1024;
@@ -614,6 +671,7 @@ static cudaError_t launch_many(const Kv8AttnArgs &a, int tiles, cudaStream_t st)
     return kv8_launch(f, dim3(tiles, a.kv.n_kv_heads, a.S), dim3(MN_THREADS), smem, st, 1, a);
 }
 
-cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tiles, cudaStream_t st) {
-    return a.kv.type == VXC_KV8_INT8 ? launch_many<VXC_KV8_INT8>(a, tiles, st) : launch_many<VXC_KV8_E4M3>(a, tiles, st);
+cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tile_q, int tiles, cudaStream_t st) {
+    return a.kv.type == VXC_KV8_INT8 ? launch_many<VXC_KV8_INT8>(a, tile_q, tiles, st)
+                                     : launch_many<VXC_KV8_E4M3>(a, tile_q, tiles, st);
 }
