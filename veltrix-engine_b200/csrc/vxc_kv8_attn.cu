@@ -547,7 +547,8 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
     } else {
         p.nq = most <= 32 ? 32 : most <= 64 ? 64 : 128;
         const long long full = (long long)n_rows * G / p.nq;
-        p.tiles = (int)(full + n_req);
+        // (a request per tile where all fit one; else tiles begin where k_kv8_attn_many says)
+        p.tiles = (int)(most <= p.nq ? n_req : full + n_req);
         p.sl_min = 512;
         const long long busy = n_req < n_rows ? n_req : n_rows;
         units = (full > busy ? full : busy) * kv->n_kv_heads;

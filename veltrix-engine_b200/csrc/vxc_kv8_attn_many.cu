@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         // every request as many as it needs; later tiles (longer contexts) first.  (One warp: the
         // same work by all of them took 2000 cycles more.)
         const int idx = (int)gridDim.x - 1 - (int)blockIdx.x;
-        int r = 0, len = a.n_req, r0, r1, pos, seq;
+        const bool one = (int)gridDim.x == a.n_req;   // a tile per request (kv8_attn_many)
+        int r = one ? idx : 0, len = one ? 1 : a.n_req, r0, r1, pos, seq;
         do {   // 32 places a step
             const int step = (len + 31) / 32, at = lane * step, ri = r + at;
             const bool in = at < len;
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 pos = in ? a.pos[ri] : 0;
                 seq = in && a.seq ? a.seq[ri] : ri;
             }
-            const bool le = in && (long long)max(r0, 0) * G / TQ + ri <= idx;
+            const bool le = in && (one || (long long)max(r0, 0) * G / TQ + ri <= idx);
             const unsigned mask = __ballot_sync(0xffffffffu, le);
             const int k = mask ? 31 - __clz(mask) : 0;
             r += k * step;
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             len = min(step, len - k * step);
         } while (true);
         const Kv8Req rq = kv8_req_of(a, seq, r0, r1, pos);
-        const long long tile0 = (long long)rq.row0 * G / TQ + r;
+        const long long tile0 = one ? idx : (long long)rq.row0 * G / TQ + r;
         if (kvh == 0 && split == 0 && lane == 0 &&
             ((rq.over && idx == tile0) || (idx == 0 && kv8_row0(a, a.n_req) > a.n_rows)))
             vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
@@ -295,7 +296,6 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     } else if (warp < MN_LOADERS / 32 + 8) {
         // ------------------------------ softmax ------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         constexpr int HC = HD / 2;   // elements of a query, columns of O per thread
         // TQ < 128: the tile's queries stand in 128 / TQ parts of its rows, and each part weighs its own
         // tokens of a tile (the others' weights are 0 there): NG groups of 16 tokens per thread
@@ -312,9 +312,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         // query srow's row and head, and how far RPS queries are
         const int t_at = (q0 + srow) / G, g_at = q0 + srow - t_at * G, t_by = RPS / G, g_by = RPS - t_by * G;
         float *xs = reinterpret_cast<float *>(sm + M::V);
-        float f;   // factor of the query's scores
-        {
-            // half a query into TMEM
+        {   // queries on their way (before the wait for registers)
             int g = g_at;
             const float *src = a.q + (size_t)(row0 + t_at) * a.ldq + (size_t)(kvh * G + g) * HD + scol;
             const long long step = (long long)t_by * a.ldq + (long long)g_by * HD, wrap = a.ldq - (long long)G * HD;
@@ -328,6 +326,11 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 if (g >= G) g -= G, src += wrap;
             }
             cp_commit();
+        }
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        float f;   // factor of the query's scores
+        {
+            // half a query into TMEM
             cp_wait<0>();
             mn_group_sync();
             float4 v[HC / 4];
@@ -517,28 +520,38 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 const int t = q / G, h = kvh * G + q - t * G;
                 *reinterpret_cast<float2 *>(a.part + (((size_t)(row0 + t) * a.H + h) * a.S + split) * (HD + 4)) = make_float2(m, L);
             }
-            mn_group_sync();
-            int g = g_at;
-            const size_t hw = ns > 1 ? (size_t)a.S * (HD + 4) : HD;   // a head's floats, a row's
-            const long long ld = ns > 1 ? (long long)a.H * hw : a.ldo;
-            float *dst = (ns > 1 ? a.part + (size_t)split * (HD + 4) + 4 : a.out) + (size_t)(row0 + t_at) * ld +
-                         (size_t)(kvh * G + g) * hw + scol;
-            const long long step = t_by * ld + (long long)(g_by * hw), wrap = ld - (long long)(G * hw);
-#pragma unroll
-            for (int i = 0; i < TQ / RPS; i++) {
-                const int rw = srow + RPS * i;
-                if (son && rw < nq - q0) {
-                    float4 x = *reinterpret_cast<const float4 *>(xs + rw * XS + scol);
-#pragma unroll
-                    for (int k = 1; k < NP; k++) {
-                        const float4 y = *reinterpret_cast<const float4 *>(xs + (rw + TQ * k) * XS + scol);
-                        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-                    }
-                    *reinterpret_cast<float4 *>(dst) = x;
+            if (NP == 1) {   // each thread sends its half row
+                fence_proxy_async();
+                if (q < nq) {
+                    const int t = q / G, h = kvh * G + q - t * G;
+                    float *to = (ns > 1 ? a.part + (((size_t)(row0 + t) * a.H + h) * a.S + split) * (HD + 4) + 4
+                                        : a.out + (size_t)(row0 + t) * a.ldo + (size_t)h * HD) + half * HC;
+                    bulk_s2g(to, smem_u32(xs + row * XS + half * HC), HC * 4);
                 }
-                dst += step;
-                g += g_by;
-                if (g >= G) g -= G, dst += wrap;
+            } else {   // the parts' sum
+                mn_group_sync();
+                int g = g_at;
+                const size_t hw = ns > 1 ? (size_t)a.S * (HD + 4) : HD;   // a head's floats, a row's
+                const long long ld = ns > 1 ? (long long)a.H * hw : a.ldo;
+                float *dst = (ns > 1 ? a.part + (size_t)split * (HD + 4) + 4 : a.out) + (size_t)(row0 + t_at) * ld +
+                             (size_t)(kvh * G + g) * hw + scol;
+                const long long step = t_by * ld + (long long)(g_by * hw), wrap = ld - (long long)(G * hw);
+#pragma unroll
+                for (int i = 0; i < TQ / RPS; i++) {
+                    const int rw = srow + RPS * i;
+                    if (son && rw < nq - q0) {
+                        float4 x = *reinterpret_cast<const float4 *>(xs + rw * XS + scol);
+#pragma unroll
+                        for (int k = 1; k < NP; k++) {
+                            const float4 y = *reinterpret_cast<const float4 *>(xs + (rw + TQ * k) * XS + scol);
+                            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                        }
+                        *reinterpret_cast<float4 *>(dst) = x;
+                    }
+                    dst += step;
+                    g += g_by;
+                    if (g >= G) g -= G, dst += wrap;
+                }
             }
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
