@@ -151,7 +151,15 @@ def test_attn_prompt(cuda, kind, hd, kh, g, lens, new):
 
 
 @pytest.mark.parametrize("kind", [INT8, E4M3])
-@pytest.mark.parametrize("hd,g,new", [(128, 8, 1), (64, 4, 3), (128, 1, 1), (128, 2, 70)])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("g,new", [(1, 16), (1, 17), (3, 8), (1, 32), (3, 11), (8, 7), (8, 8), (5, 13), (1, 127), (16, 8), (3, 43)])
+def test_attn_around_the_tile_sizes(cuda, kind, hd, g, new):
+    """16, 32, 64 and 128 queries per kv head, one less and a few more; requests of fewer rows."""
+    check_attn(cuda, kind, hd, 2, g, 48, [0, 3, 90, 333], [new, 1, new - 1, new])
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+@pytest.mark.parametrize("hd,g,new", [(128, 8, 1), (64, 4, 3), (128, 1, 1), (128, 2, 70), (128, 2, 13), (96, 8, 7)])
 def test_attn_long_context_is_split_and_joined(cuda, kind, hd, g, new):
     check_attn(cuda, kind, hd, 1, g, 64, [5000, 0, 2047], [new, new, new])
 
@@ -170,14 +178,14 @@ def test_attn_requests_without_rows_and_rows_without_tokens(cuda):
     assert np.all(got[:2] == 0) and np.any(got[2] != 0)
 
 
-@pytest.mark.parametrize("hd,new", [(128, 1), (64, 5), (128, 80)])
+@pytest.mark.parametrize("hd,new", [(128, 1), (64, 5), (128, 80), (128, 11), (96, 25), (32, 31)])
 def test_attn_strides_and_spare_rows(cuda, hd, new):
     check_attn(cuda, E4M3, hd, 2, 2, 32, [50, 7], [new, new], ld_pad=12)
     # the caller's n_rows and max_new are upper bounds
     check_attn(cuda, E4M3, hd, 2, 2, 32, [50, 7], [new, new], n_rows=2 * new + 3, most=new + 11)
 
 
-@pytest.mark.parametrize("new", [1, 6, 90])
+@pytest.mark.parametrize("new", [1, 6, 14, 90])
 def test_attn_bytes_behind_the_last_token_are_not_used(cuda, new):
     torch = cuda
     rng = np.random.default_rng(5)
@@ -199,7 +207,7 @@ def test_attn_bytes_behind_the_last_token_are_not_used(cuda, new):
 
 
 @pytest.mark.parametrize("kind", [INT8, E4M3])
-@pytest.mark.parametrize("new", [1, 5, 70])
+@pytest.mark.parametrize("new", [1, 5, 14, 70])
 def test_attn_scales_of_any_size(cuda, kind, new):
     """Blocks whose scales are far apart, zero among them, and far from 1; queries far from 1."""
     torch = cuda
@@ -220,7 +228,7 @@ def test_attn_scales_of_any_size(cuda, kind, new):
     assert np.all(np.abs(got - want) <= bound + 2.0 ** -30 * np.abs(want).max())
 
 
-@pytest.mark.parametrize("new", [1, 4, 66])
+@pytest.mark.parametrize("new", [1, 4, 12, 30, 66])
 def test_attn_bad_table_entries_are_masked_and_reported(cuda, new):
     rng = np.random.default_rng(2)
     table, nb = paged(rng, [90 + new, 20 + new], 16)
@@ -234,7 +242,7 @@ def test_attn_bad_table_entries_are_masked_and_reported(cuda, new):
     assert np.all(np.abs(got - want) <= bound)
 
 
-@pytest.mark.parametrize("new", [2, 70])
+@pytest.mark.parametrize("new", [2, 12, 30, 70])
 def test_attn_lengths_beyond_the_arguments_are_reported(cuda, new):
     rng = np.random.default_rng(2)
     table, nb = paged(rng, [100 + new], 16)
