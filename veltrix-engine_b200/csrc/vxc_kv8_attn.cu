@@ -549,10 +549,25 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         const long long full = (long long)n_rows * G / p.nq;
         // (a request per tile where all fit one; else tiles begin where k_kv8_attn_many says)
         p.tiles = (int)(most <= p.nq ? n_req : full + n_req);
-        p.sl_min = 512;
+        p.sl_min = 256;
         const long long busy = n_req < n_rows ? n_req : n_rows;
-        units = (full > busy ? full : busy) * kv->n_kv_heads;
-        S = units >= 2 * 148 ? 1 : (3 * 148 + units - 1) / units;
+        const long long some = ((long long)n_rows * G + p.nq - 1) / p.nq;
+        units = (some > busy ? some : busy) * kv->n_kv_heads;
+        // A CTA costs about 11 us and 1.86 us per 128 tokens, one fits an SM; the join 3 us and its
+        // records' way.  The S of the least time, as long as the longest CTA and as all of them on
+        // 148 SMs: requests begin longest first and have 0.6 of the tokens on average; a single one has
+        // them all, and then CTAs come in whole rounds.  Measured (us, S = 1, 2, ...): 96 units of 8192
+        // tokens 129, 78, 83; 64 units 128, 76, 59, 58, 62; 256 units of 4096 89, 112, 123; 200 units of
+        // 16384 255, 212, 219; 128 units of 2000 39, 44, 54.
+        double best = 0;
+        S = 1;
+        for (int i = 1; i <= 64; i++) {
+            const double cta = 11 + 0.0145 * tokens / i;
+            const double all = n_req == 1 ? (units * i + 147) / 148 * cta : units * (11.0 * i + 0.6 * 0.0145 * tokens) / 148;
+            const double join = i == 1 ? 0 : 3 + 2e-6 * n_rows * n_heads * i * (kv->head_dim + 4);
+            const double time = (cta > all ? cta : all) + join;
+            if (i == 1 || time < best) best = time, S = i;
+        }
     }
     const long long need = (tokens + p.sl_min - 1) / p.sl_min;
     if (S > need) S = need;
@@ -605,10 +620,14 @@ static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st)
     a.S = p.S;
     a.sl_min = p.sl_min;
     a.pages = p.pages;
+    // (where all CTAs fit the GPU at once the order is of no use)
+    const bool many = p.nq > ATTN_FEW_MAX;
+    a.ranked = many && p.tiles == a.n_req && a.n_req > 1 && a.n_req <= KV8_RANKED &&
+               (long long)a.n_req * a.kv.n_kv_heads * p.S > 148;
     a.err = vxc_device_error_ptr();
     const vxc_kv8 *kv = &a.kv;
     const int hd = kv->head_dim;
-    if (p.nq > ATTN_FEW_MAX) {
+    if (many) {
         VXC_CUDA_OK(kv8_attn_many(a, p.nq, p.tiles, st));
     } else {
         attn_kernel_t f = kv->type == VXC_KV8_INT8 ? few_kernel<VXC_KV8_INT8>(hd, p.nq) : few_kernel<VXC_KV8_E4M3>(hd, p.nq);

@@ -133,14 +133,16 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     __shared__ __align__(16) float page_ks[MN_PAGES][8], page_vs[MN_PAGES][8], page_lv[MN_PAGES][8];
     __shared__ float2 red[2][2][128];              // [tile parity][half][query]: maxima of half a tile
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, pos_s[KV8_RANKED];
     __shared__ struct {
         const int *table;
         int q0, nq, row0, pos, kvlen, ns, SL;   // nq 0: no work
     } item;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    // heads and splits of a tile stand together: tiles begin in their order, over the whole grid
+    const int tiles = (int)gridDim.x / (KH * a.S), tile = (int)blockIdx.x / (KH * a.S);
+    const int kvh = ((int)blockIdx.x - tile * KH * a.S) / a.S, split = ((int)blockIdx.x - tile * KH * a.S) % a.S;
     const uint32_t bar0 = smem_u32(bars);
     auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (loaders)
     auto vfull = [&](int s) { return bar0 + 8u * (2 + s); };
@@ -168,8 +170,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         // request and query tile: tiles of request r begin at floor(row0 G / TQ) + r, which leaves
         // every request as many as it needs; later tiles (longer contexts) first.  (One warp: the
         // same work by all of them took 2000 cycles more.)
-        const int idx = (int)gridDim.x - 1 - (int)blockIdx.x;
-        const bool one = (int)gridDim.x == a.n_req;   // a tile per request (kv8_attn_many)
+        const bool one = tiles == a.n_req;   // a tile per request
+        const int idx = a.ranked ? kv8_ranked(a, tile, pos_s) : tiles - 1 - tile;
         int r = one ? idx : 0, len = one ? 1 : a.n_req, r0, r1, pos, seq;
         do {   // 32 places a step
             const int step = (len + 31) / 32, at = lane * step, ri = r + at;
@@ -681,7 +683,7 @@ static cudaError_t launch_many(const Kv8AttnArgs &a, int tile_q, int tiles, cuda
     if (smem < 116 * 1024) smem = 116 * 1024;
     cudaError_t e = kv8_allow_smem((const void *)f, smem);
     if (e != cudaSuccess) return e;
-    return kv8_launch(f, dim3(tiles, a.kv.n_kv_heads, a.S), dim3(MN_THREADS), smem, st, 1, a);
+    return kv8_launch(f, dim3((unsigned)(tiles * a.kv.n_kv_heads * a.S)), dim3(MN_THREADS), smem, st, 1, a);
 }
 
 cudaError_t kv8_attn_many(const Kv8AttnArgs &a, int tile_q, int tiles, cudaStream_t st) {
