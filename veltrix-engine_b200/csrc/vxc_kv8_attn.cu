@@ -83,12 +83,13 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     constexpr int NT = HD / 8;                 // column tiles of the output
     constexpr int TILE = HD * 32;              // bytes of K and V of 16 tokens
     constexpr int STAGE = 2 * TILE;
-    extern __shared__ __align__(16) unsigned char sm[];
+    extern __shared__ __align__(128) unsigned char sm[];
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int KH = a.kv.n_kv_heads, G = a.H / KH, bs = a.kv.block_size;
     pdl_trigger();
     pdl_wait();
-    const int r = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    // (scratch in the ring: static shared memory would move the ring off its 128-byte lines, +6 %)
+    const int r = a.ranked ? kv8_ranked(a, blockIdx.z, reinterpret_cast<int *>(sm)) : blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
     const Kv8Req rq = kv8_req(a, r);
     if (rq.over && kvh == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
     const int nq = rq.T * G;   // at most NQ
@@ -473,27 +474,37 @@ __global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
     // only the splits that begin at or before the row's own token hold anything
     const int live = min(ns, (rq.pos + (i - rq.row0)) / SL + 1);
     const float *rec = a.part + ((size_t)i * a.H + h) * a.S * (HD + 4);
-    float M = -INFINITY, L = 0.0f, o[HD / 32];
+    // lanes have a record's {m, l} each; then, of one record after the other, four values each
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int n = rq.pos + (i - rq.row0) >= 0 ? live : 0;
+    float2 ml[2];
 #pragma unroll
-    for (int d = 0; d < HD / 32; d++) o[d] = 0.0f;
-    if (rq.pos + (i - rq.row0) >= 0) {
-        for (int s = 0; s < live; s++) M = fmaxf(M, rec[(size_t)s * (HD + 4)]);
-#pragma unroll 4
-        for (int s = 0; s < live; s++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(rec + (size_t)s * (HD + 4));
-            const float e = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-            L = fmaf(e, ml.y, L);
+    for (int k = 0; k < 2; k++) {
+        const int s = lane + 32 * k;   // S is at most 64
+        ml[k] = s < n ? *reinterpret_cast<const float2 *>(rec + (size_t)s * (HD + 4)) : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, ml[k].x);
+    }
 #pragma unroll
-            for (int d = 0; d < HD / 32; d++) {
-                const float x = rec[(size_t)s * (HD + 4) + 4 + d * 32 + lane];
-                o[d] = fmaf(e, e != 0.0f ? x : 0.0f, o[d]);
-            }
-        }
+    for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        ml[k].x = ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - M);
+        L = fmaf(ml[k].x, ml[k].y, L);
+    }
+#pragma unroll
+    for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+    const float *mine = rec + 4 + 4 * min(lane, HD / 4 - 1);
+#pragma unroll 8
+    for (int s = 0; s < n; s++) {
+        const float e = __shfl_sync(0xffffffffu, s < 32 ? ml[0].x : ml[1].x, s & 31);
+        const float4 x = *reinterpret_cast<const float4 *>(mine + (size_t)s * (HD + 4));
+        if (e != 0.0f) o.x = fmaf(e, x.x, o.x), o.y = fmaf(e, x.y, o.y), o.z = fmaf(e, x.z, o.z), o.w = fmaf(e, x.w, o.w);
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
-    float *out = a.out + (size_t)i * a.ldo + (size_t)h * HD;
-#pragma unroll
-    for (int d = 0; d < HD / 32; d++) out[d * 32 + lane] = o[d] * inv;
+    if (lane < HD / 4)
+        *reinterpret_cast<float4 *>(a.out + (size_t)i * a.ldo + (size_t)h * HD + 4 * lane) =
+            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
@@ -532,18 +543,23 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         p.nq = most <= 8 ? 8 : 16;
         p.tiles = 0;
         units = (long long)n_req * kv->n_kv_heads;
-        // A CTA costs about 3.5 us besides its tokens (1.4 us for 128), two fit an SM.  So: as many
-        // splits as fit the GPU at once, none shorter than the cost warrants (128 tokens for a few
-        // units, 1024 for 256 of them); more only to even out long contexts (4096 tokens).  Measured:
-        // 256 units of 768 tokens 13.5 us whole, 17.5 in two; 264 units of up to 16384 162 us whole,
-        // 122 in four, 152 in eight; 32 units of 768 9.2 us whole, 7.3 in six.
-        const long long wide = units / 32 < 1 ? 1 : units / 32 > 32 ? 32 : units / 32;
-        p.sl_min = (int)(128 * wide);
-        S = 2 * 148 / units;
-        const long long even = (tokens + 4095) / 4096;
-        // above 8 a second kernel joins the splits: worth it for long ones only
-        if (S > 8 && tokens <= 8 * 512) S = 8;
-        if (S < even) S = even;
+        // A CTA costs about 4 us besides its tokens and, joined by a cluster, 2 us more; two fit an SM, and
+        // each further CTA of a unit takes 12 us of a place (a cluster's CTAs begin and end together); above
+        // 8 a second kernel joins them.  The S of the least time, as below; measured (us, S = 1, 2, ...):
+        // 256 units of 768 tokens 13.5, 17.5; 256 of 4096 58, 47, 53; 512 of 8192 108, 127, 157; 800 of
+        // 4096 105, 136, 146; 264 of 16384 -, 105, 120, 138; 32 of 768 9.2, in six 7.3.
+        p.sl_min = 128;
+        double best = 0;
+        const double byte = kv->head_dim / 128.0;
+        S = 1;
+        for (int i = 1; i <= 64; i++) {
+            const double cta = 4 + 0.0125 * byte * tokens / i + (i == 1 ? 0 : i <= 8 ? 2 : 8);
+            const double places = i <= 8 ? 4 + 12.0 * (i - 1) : 6.0 * i;
+            const double all = n_req == 1 ? (units * i + 295) / 296 * cta
+                                          : units * (places + 0.5 * 0.0144 * byte * tokens) / 296 + 0.25 * cta;
+            const double time = cta > all || units * i <= 296 ? cta : all;
+            if (i == 1 || time < best) best = time, S = i;
+        }
     } else {
         p.nq = most <= 32 ? 32 : most <= 64 ? 64 : 128;
         const long long full = (long long)n_rows * G / p.nq;
@@ -620,10 +636,10 @@ static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st)
     a.S = p.S;
     a.sl_min = p.sl_min;
     a.pages = p.pages;
-    // (where all CTAs fit the GPU at once the order is of no use)
+    // (where all CTAs fit the GPU at once, one or two per SM, the order is of no use)
     const bool many = p.nq > ATTN_FEW_MAX;
-    a.ranked = many && p.tiles == a.n_req && a.n_req > 1 && a.n_req <= KV8_RANKED &&
-               (long long)a.n_req * a.kv.n_kv_heads * p.S > 148;
+    a.ranked = (!many || p.tiles == a.n_req) && a.n_req > 1 && a.n_req <= KV8_RANKED &&
+               (long long)a.n_req * a.kv.n_kv_heads * p.S > (many ? 148 : 2 * 148);
     a.err = vxc_device_error_ptr();
     const vxc_kv8 *kv = &a.kv;
     const int hd = kv->head_dim;

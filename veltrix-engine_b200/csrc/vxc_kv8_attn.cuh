@@ -2,6 +2,7 @@
 // share: their arguments, a request's bounds, and the arithmetic of codes,
 // queries and weights.
 #pragma once
+#include <limits.h>
 #include "vxc_kv8.cuh"
 
 struct Kv8AttnArgs {
@@ -21,7 +22,7 @@ struct Kv8AttnArgs {
     float *part;        // records of the splits
     int S, sl_min;      // splits per request at most, tokens per split at least
     int pages;          // blocks a split may touch, rounded up to 4 (k_kv8_attn_few)
-    int ranked;         // k_kv8_attn_many: requests begin by length, longest first (at most KV8_RANKED)
+    int ranked;         // requests begin by length, longest first (at most KV8_RANKED)
     unsigned int *err;
 };
 
@@ -119,31 +120,27 @@ __device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
     return kv8_req_of(a, a.seq ? a.seq[r] : r, kv8_row0(a, r), kv8_row0(a, r + 1), a.pos[r]);
 }
 
-// k_kv8_attn_many begins requests longest first: what begins last is then short.  (32 requests of 7 rows
-// behind up to 4096 tokens: 122 -> 112 us.  k_kv8_attn_few, whose CTAs are shorter, gained nothing.)  The
-// position is length enough.
+// Requests begin longest first where not all CTAs fit the GPU at once, so that what begins last is short.
+// (33 requests of one row behind up to 16384 tokens: 124 -> 100 us; 32 of 7 rows behind up to 4096:
+// 122 -> 112 us.)  The position is length enough.
 #define KV8_RANKED 128
-// Called by warp 0: the request whose position is the k-th largest; pos_s: KV8_RANKED ints of shared memory.
+// The request whose position is the k-th largest.  Called by every thread of a block of at least KV8_RANKED;
+// pos_s: KV8_RANKED + 1 ints of shared memory, 16-byte aligned.
 __device__ __forceinline__ int kv8_ranked(const Kv8AttnArgs &a, int k, int *pos_s) {
-    const int lane = threadIdx.x & 31, n = a.n_req;
-    int key[KV8_RANKED / 32], rank[KV8_RANKED / 32], found = 0;
-#pragma unroll
-    for (int i = 0; i < KV8_RANKED / 32; i++) {
-        const int r = lane + 32 * i;
-        key[i] = r < n ? a.pos[r] : 0;
-        rank[i] = 0;
-        if (r < n) pos_s[r] = key[i];
+    const int me = threadIdx.x, n = a.n_req, key = me < n ? a.pos[me] : INT_MIN;
+    if (me < KV8_RANKED) pos_s[me] = key;
+    __syncthreads();
+    if (me < n) {
+        int rank = 0;
+        auto count = [&](int p, int o) { rank += p > key || (p == key && o < me); };
+        for (int o = 0; o < n; o += 4) {   // (INT_MIN behind the last: counts for nobody)
+            const int4 p = *reinterpret_cast<const int4 *>(pos_s + o);
+            count(p.x, o), count(p.y, o + 1), count(p.z, o + 2), count(p.w, o + 3);
+        }
+        if (rank == k) pos_s[KV8_RANKED] = me;
     }
-    __syncwarp();
-    for (int o = 0; o < n; o++) {
-        const int p = pos_s[o];
-#pragma unroll
-        for (int i = 0; i < KV8_RANKED / 32; i++) rank[i] += p > key[i] || (p == key[i] && o < lane + 32 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < KV8_RANKED / 32; i++)
-        if (lane + 32 * i < n && rank[i] == k) found = lane + 32 * i + 1;
-    return (int)__reduce_max_sync(0xffffffffu, (unsigned)found) - 1;
+    __syncthreads();
+    return pos_s[KV8_RANKED];
 }
 
 // Splits of a request: enough for SL_min tokens each, at most S.
