@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     pdl_trigger();
     pdl_wait();
     // (scratch in the ring: static shared memory would move the ring off its 128-byte lines, +6 %)
-    const int r = a.ranked ? kv8_ranked(a, blockIdx.z, reinterpret_cast<int *>(sm)) : blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    const int r = a.ranked ? kv8_ranked<128>(a, blockIdx.z, reinterpret_cast<int *>(sm)) : blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
     const Kv8Req rq = kv8_req(a, r);
     if (rq.over && kvh == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
     const int nq = rq.T * G;   // at most NQ
