@@ -360,6 +360,8 @@ size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, i
  * 4); out may not overlap q.  Products are exact to fp32 level: codes are
  * exact in fp16, queries and weights are split into two fp16 parts, sums and
  * softmax are fp32.
+ * (n_rows <= VXC_KV8_MAX_ROWS, n_rows * n_heads < 2^31, max_blocks * block_size
+ * <= 2^30.)
  * A row whose position is negative sees no token and is set to 0.  Rows behind
  * d_row0[n_req] are left as they were.  Bytes of the cache behind a request's
  * last token are not used, whatever they hold.  These raise the device error

@@ -61,6 +61,7 @@ def test_append_refusals(bad):
                                  dict(table=None), dict(row0=None), dict(pos=None), dict(q=BUF + 4), dict(out=BUF + 8),
                                  dict(ldq=252), dict(ldo=100), dict(ldq=258), dict(n_req=0), dict(n_req=8193),
                                  dict(n_rows=-1), dict(n_rows=(1 << 22) + 1), dict(most=0), dict(mb=0), dict(mb=1 << 28),
+                                 dict(n_rows=1 << 20, h=2048, ldq=1 << 20, ldo=1 << 20),
                                  dict(scale=float("nan")), dict(scale=float("inf"))], ids=str)
 def test_attn_refusals(bad):
     assert attn(cache(), **bad) == PARAM

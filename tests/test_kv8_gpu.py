@@ -164,9 +164,19 @@ def test_attn_long_context_is_split_and_joined(cuda, kind, hd, g, new):
     check_attn(cuda, kind, hd, 1, g, 64, [5000, 0, 2047], [new, new, new])
 
 
+def test_attn_context_of_over_half_a_million_tokens(cuda):
+    """More than 64 splits of 8192 tokens."""
+    check_attn(cuda, INT8, 32, 1, 2, 256, [600000, 40], [1, 1])
+    check_attn(cuda, E4M3, 32, 1, 1, 256, [550000], [33])
+
+
 def test_attn_many_requests(cuda):
     rng = np.random.default_rng(3)
     check_attn(cuda, INT8, 64, 2, 2, 16, rng.integers(0, 70, 300).tolist(), rng.integers(0, 3, 300).tolist())
+    # begun by length: equal ones, 128 and one more
+    for n, new in ((128, 1), (129, 1), (128, 20), (129, 20), (5, 9)):
+        check_attn(cuda, INT8, 32, 4, 3, 16, rng.integers(0, 4, n).tolist(), [new] * n)
+    check_attn(cuda, INT8, 32, 40, 3, 16, [7] * 9, [9] * 9)
 
 
 def test_attn_requests_without_rows_and_rows_without_tokens(cuda):

@@ -474,33 +474,29 @@ __global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
     // only the splits that begin at or before the row's own token hold anything
     const int live = min(ns, (rq.pos + (i - rq.row0)) / SL + 1);
     const float *rec = a.part + ((size_t)i * a.H + h) * a.S * (HD + 4);
-    // lanes have a record's {m, l} each; then, of one record after the other, four values each
+    const int n = rq.pos + (i - rq.row0) >= 0 ? live : 0;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const int n = rq.pos + (i - rq.row0) >= 0 ? live : 0;
-    float2 ml[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int s = lane + 32 * k;   // S is at most 64
-        ml[k] = s < n ? *reinterpret_cast<const float2 *>(rec + (size_t)s * (HD + 4)) : make_float2(-INFINITY, 0.0f);
-        M = fmaxf(M, ml[k].x);
-    }
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, rec[(size_t)s * (HD + 4)]);
 #pragma unroll
     for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        ml[k].x = ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - M);
-        L = fmaf(ml[k].x, ml[k].y, L);
+    // lanes have a record's {m, l} each, then, of one record after the other, four values each
+    const float *mine = rec + 4 + 4 * min(lane, HD / 4 - 1);
+    for (int at = 0; at < n; at += 32) {
+        const int some = min(n - at, 32);
+        const float2 ml = lane < some ? *reinterpret_cast<const float2 *>(rec + (size_t)(at + lane) * (HD + 4))
+                                      : make_float2(-INFINITY, 0.0f);
+        const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        L = fmaf(w, ml.y, L);
+#pragma unroll 8
+        for (int s = 0; s < some; s++) {
+            const float e = __shfl_sync(0xffffffffu, w, s);
+            const float4 x = *reinterpret_cast<const float4 *>(mine + (size_t)(at + s) * (HD + 4));
+            if (e != 0.0f) o.x = fmaf(e, x.x, o.x), o.y = fmaf(e, x.y, o.y), o.z = fmaf(e, x.z, o.z), o.w = fmaf(e, x.w, o.w);
+        }
     }
 #pragma unroll
     for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-    const float *mine = rec + 4 + 4 * min(lane, HD / 4 - 1);
-#pragma unroll 8
-    for (int s = 0; s < n; s++) {
-        const float e = __shfl_sync(0xffffffffu, s < 32 ? ml[0].x : ml[1].x, s & 31);
-        const float4 x = *reinterpret_cast<const float4 *>(mine + (size_t)s * (HD + 4));
-        if (e != 0.0f) o.x = fmaf(e, x.x, o.x), o.y = fmaf(e, x.y, o.y), o.z = fmaf(e, x.z, o.z), o.w = fmaf(e, x.w, o.w);
-    }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
     if (lane < HD / 4)
         *reinterpret_cast<float4 *>(a.out + (size_t)i * a.ldo + (size_t)h * HD + 4 * lane) =
@@ -514,7 +510,8 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
         return -4;
     }
     if (n_req < 1 || n_req > VXC_KV8_MAX_REQ || n_rows < 0 || n_rows > VXC_KV8_MAX_ROWS || max_new < 1 ||
-        max_blocks < 1 || (long long)max_blocks * kv->block_size > KV8_MAX_TOKENS) {
+        max_blocks < 1 || (long long)max_blocks * kv->block_size > KV8_MAX_TOKENS ||
+        (long long)n_rows * n_heads > INT_MAX) {
         vxc_set_error("vxc_kv8_attn: %d requests, %d rows (%d of one request), %d blocks per request", n_req, n_rows,
                       max_new, max_blocks);
         return -4;
@@ -602,11 +599,14 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
 // Whether the splits leave records for k_kv8_attn_join.
 static bool attn_records(const AttnPlan &p) { return p.S > (p.nq > ATTN_FEW_MAX ? 1 : 8); }
 
+static size_t attn_need(const vxc_kv8 *kv, int n_heads, int n_rows, const AttnPlan &p) {
+    return attn_records(p) ? (size_t)n_rows * n_heads * p.S * (kv->head_dim + 4) * sizeof(float) : 0;
+}
+
 extern "C" size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new,
                                                int max_blocks) {
     if (attn_check(kv, n_heads, n_req, n_rows, max_new, max_blocks)) return 0;
-    const AttnPlan p = attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks);
-    return attn_records(p) ? (size_t)n_rows * n_heads * p.S * (kv->head_dim + 4) * sizeof(float) : 0;
+    return attn_need(kv, n_heads, n_rows, attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks));
 }
 
 typedef void (*attn_kernel_t)(const Kv8AttnArgs);
@@ -676,7 +676,7 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
         return -4;
     }
     const AttnPlan p = attn_plan(kv, n_heads, n_req, n_rows, max_new, max_blocks);
-    const size_t need = vxc_kv8_attn_workspace_bytes(kv, n_heads, n_req, n_rows, max_new, max_blocks);
+    const size_t need = attn_need(kv, n_heads, n_rows, p);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) {
         vxc_set_error("vxc_kv8_attn: workspace of %zu bytes needed (16-byte aligned)", need);
         return -4;

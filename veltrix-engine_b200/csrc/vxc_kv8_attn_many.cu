@@ -679,6 +679,7 @@ static cudaError_t launch_many(const Kv8AttnArgs &a, int tile_q, int tiles, cuda
         case 96: f = many_kernel<TYPE, 96>(tile_q); smem = MnSmem<96>::BYTES; break;
         default: f = many_kernel<TYPE, 128>(tile_q); smem = MnSmem<128>::BYTES; break;
     }
+    if ((long long)tiles * a.kv.n_kv_heads * a.S > INT_MAX) return cudaErrorInvalidValue;
     // TMEM is allocated whole: one CTA per SM, so at least half of the shared memory is asked for
     if (smem < 116 * 1024) smem = 116 * 1024;
     cudaError_t e = kv8_allow_smem((const void *)f, smem);
