@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         float acc[HC];
 #pragma unroll
         for (int d = 0; d < HC; d++) acc[d] = 0.0f;
-        const int lim = q < nq ? pos + q / G : -1;
+        // (places without a query: as the last one, so that they do not cost their warp the masks)
+        const int lim = pos + min(q, nq - 1) / G;
         // adds O of tile j to the registers
         auto drain = [&](int j) -> bool {
             const bool ok = mn_wait(ofull(j & 1), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
@@ -416,6 +417,12 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             const bool whole = __all_sync(0xffffffffu, lim >= t0 + 16 * NG - 1) && bad == 0;
             tmem_wait_ld();
             tmem_pin<16 * NG>(v);
+            if (NP > 1) {
+                const uint32_t none[16] = {};
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    if (g / NG != part) tmem_st16(t_s + 16 * g, none);
+            }
             if (!whole) {
 #pragma unroll
                 for (int c = 0; c < NG; c++) {   // visible tokens of group c: the low bits of a mask
@@ -481,12 +488,6 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 }
                 // hi in columns 0-7 of the group's 16, lo in 8-15
                 tmem_st16(t_g + 16 * c, w);
-            }
-            if (NP > 1) {
-                const uint32_t none[16] = {};
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                    if (g / NG != part) tmem_st16(t_s + 16 * g, none);
             }
             {
                 float x, y;
