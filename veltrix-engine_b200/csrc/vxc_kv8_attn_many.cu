@@ -19,33 +19,39 @@
 // shared memory added half of that: hence in TMEM.)
 //
 // Roles (640 threads, one CTA per SM):
-//   warps 0-7    loaders: cp.async 8-bit rows into slots of each thread's own
-//                (MN_AHEAD pieces ahead), convert, store fp16 core matrices
+//   warps 0-7    loaders: convert raw rows to fp16 core matrices
 //   warps 8-15   softmax, two threads per query: warps 8-11 have tokens 0-63 of
 //                a tile and the first half of the output columns, warps 12-15
 //                the others; they exchange their maxima through shared memory.
 //                Weights of tile j first, then O of tile j - 1 is added, so its
-//                product runs beside them
+//                product runs beside them.  In tiles of 64 or 32 queries the
+//                queries stand in 2 or 4 copies, which share a tile's tokens
 //   warp 16      issues S of tile j + 2; warp 17 issues P V of tile j
 //   warp 18      block table and scales of the coming tiles, four at a time
-//   warp 19      nothing: registers are shared out by fours of warps
+//   warp 19      bulk copies of raw rows, a span of 16 tokens each, MN_AHEAD
+//                pieces (K or V of a tile) ahead
 // TMEM: two buffers of 128 columns for S / P, 128 for O, 128 for Q.
 // K and V tiles have two slots each.  K as [head dim chunk][token] x 16 bytes
 // is K-major, V in the same layout is MN-major; chunks are 2064 bytes apart, so
-// the loaders' 16-byte stores fall into different banks.  Queries and outputs
-// go through shared memory, 16 columns at a time, so that an instruction
-// touches 8 lines instead of 32 (queries read a lane per row: 5 us a CTA).
+// the loaders' 16-byte stores fall into different banks.  Queries come and
+// outputs go as whole rows, through V's slots before and after their use.
 //
-// Measured (32 query heads of 128 over 8 kv heads): 8192 rows behind 8192
-// tokens of one request 3.43 ms, 561 Tflop/s of attention = 1.12 Pflop/s of
-// fp16 products, 68 % of what a dense bf16 product reaches; 8 prompts of 512
-// rows 122 us; 32 requests of 7 rows behind 4096 tokens 150 us (28 of a tile's
-// 128 queries exist).  Bound: the softmax warps' instructions (scores are read,
-// multiplied, exponentiated, split in two and stored), tensor pipe busy half of
-// the time.  Slower: one thread per query, -9 %; each half of the softmax
-// warps on a tile of its own, -5 to -10 %; persistent CTAs over a list of
-// tiles, -20 %; 128 loader threads; queries in shared memory; warps that skip
-// their arithmetic when none of their queries exist, -6 %.
+// Measured (heads of 128): 4096 rows behind 12288 tokens, 64 heads over 8,
+// 3.35 ms: 575 Tflop/s of attention, 1.15 Pflop/s of fp16 products, 0.69 of a
+// library's bf16 product.  8 prompts of up to 512 rows, 32 heads, 97 us; 32
+// requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 87 us.  Bound:
+// a tile takes 3700 cycles, of which 2048 are products.  The softmax warps'
+// chain is as long: waiting for and reading S 900, maxima 400, weights 1800 (64
+// of each thread's exponentials and conversions share a unit of 16 lanes), O
+// 450, and the next product starts behind it (one O fits TMEM).  A CTA costs
+// 11 us besides, mostly latencies one after the other: lookups, queries, first
+// tile, last product, output; hence short requests' distance from their floor.
+// Slower: one thread per query (-9 %); each half of the softmax warps on a tile
+// of its own (-5 to -10 %); persistent CTAs over a list of tiles (-20 %); 128
+// loader threads; queries as operands from shared memory; O added beside or
+// before the weights (-15 to -40 %: TMEM reads queue behind its stores); loaders
+// with cp.async of their own (they were the longest chain, 3750 cycles a tile);
+// arrivals of threads instead of warps.
 // Every wait is bounded (VXC_WAIT_NS); on expiry the error word is set, every
 // role leaves its loop, and TMEM is freed after the issued work has ended.
 #include "vxc_kv8_attn.cuh"
@@ -59,7 +65,7 @@
 template <int HD>
 struct MnSmem {
     static constexpr int TILE = HD / 8 * MN_CHUNK;          // one fp16 tile of 128 rows
-    static constexpr int PIECE = 128 * (HD == 96 ? 128 : HD);   // raw bytes of one (96: as 8 units per row)
+    static constexpr int PIECE = 128 * HD;                  // its bytes as they come from the cache
     // V's tiles, before them the queries and after them the outputs: 128 rows of HD + 4 floats
     static constexpr int QO = 128 * (HD + 4) * 4, VQO = 2 * TILE > QO ? 2 * TILE : QO;
     static constexpr int K = 0, RAW = 2 * TILE, V = RAW + MN_AHEAD * PIECE, BYTES = V + VQO;
@@ -119,6 +125,14 @@ __device__ __forceinline__ float mn_factor(float x) { return fmaxf(x, 1e-37f); }
 // The softmax warps only.
 __device__ __forceinline__ void mn_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// One lane of the (whole) warp, the same one each time: products and their commits are one thread's.  (With
+// `lane == 0` instead the compiler does not see that one thread runs, and each product took 100 cycles to issue.)
+__device__ __forceinline__ bool mn_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // Every warp, at the end of its role.  Registers go back to what the block was launched with only behind
 // this: a warp that is done early (one has nothing to do at all) would otherwise take back registers that a
 // softmax warp has not got yet, and that warp would wait for them for ever.
@@ -128,7 +142,7 @@ template <int TYPE, int HD, int TQ>
 __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnArgs a) {
     using M = MnSmem<HD>;
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ __align__(8) uint64_t bars[18 + 2 * MN_PAGES];
+    __shared__ __align__(8) uint64_t bars[18 + 2 * MN_PAGES + MN_AHEAD];
     __shared__ long long page_at[MN_PAGES][8];     // byte offset of a 16-token group in the cache; -1 none, -2 bad block
     __shared__ __align__(16) float page_ks[MN_PAGES][8], page_vs[MN_PAGES][8], page_lv[MN_PAGES][8];
     __shared__ float2 red[2][2][128];              // [tile parity][half][query]: maxima of half a tile
@@ -144,23 +158,27 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     const int tiles = (int)gridDim.x / (KH * a.S), tile = (int)blockIdx.x / (KH * a.S);
     const int kvh = ((int)blockIdx.x - tile * KH * a.S) / a.S, split = ((int)blockIdx.x - tile * KH * a.S) % a.S;
     const uint32_t bar0 = smem_u32(bars);
-    auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (loaders)
+    // warps arrive, not threads: 32 arrivals are 32 atomics on one word
+    auto kfull = [&](int s) { return bar0 + 8u * s; };             // K tile stored (loader warps)
     auto vfull = [&](int s) { return bar0 + 8u * (2 + s); };
+    auto rfull = [&](int s) { return bar0 + 8u * (4 + s); };       // raw piece landed (bytes)
     auto sfull = [&](int b) { return bar0 + 8u * (8 + b); };       // S product of a tile in buffer b done: its K slot is free
-    auto pfull = [&](int b) { return bar0 + 8u * (10 + b); };      // its weights stored (256 threads)
+    auto pfull = [&](int b) { return bar0 + 8u * (10 + b); };      // its weights stored (softmax warps)
     auto ofull = [&](int b) { return bar0 + 8u * (12 + b); };      // its P V product done: its V slot is free
-    const uint32_t oempty = bar0 + 8u * 14, qfull = bar0 + 8u * 15;   // O read; queries stored (256 threads)
-    auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks and scales of a tile (8 lanes)
-    auto gempty = [&](int s) { return bar0 + 8u * (26 + s); };     // loaders (after V) and the softmax group are done with them
-    pdl_trigger();
+    const uint32_t oempty = bar0 + 8u * 14, qfull = bar0 + 8u * 15;   // O read; queries stored (softmax warps)
+    auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks and scales of a tile
+    auto gempty = [&](int s) { return bar0 + 8u * (18 + MN_PAGES + s); };   // the copy warp and the softmax warps are done with them
+    auto rempty = [&](int s) { return bar0 + 8u * (18 + 2 * MN_PAGES + s); };   // raw piece read (loader warps)
+    static_assert(MN_AHEAD <= 4, "rfull has places 4-7");
     if (tid == 32) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(kfull(s), MN_LOADERS), mbar_init(vfull(s), MN_LOADERS);
-            mbar_init(sfull(s), 1), mbar_init(pfull(s), 256), mbar_init(ofull(s), 1);
+            mbar_init(kfull(s), MN_LOADERS / 32), mbar_init(vfull(s), MN_LOADERS / 32);
+            mbar_init(sfull(s), 1), mbar_init(pfull(s), 8), mbar_init(ofull(s), 1);
             mbar_init(bar0 + 8u * (16 + s), 1);   // an issuer's last work, after an abort
         }
-        mbar_init(oempty, 256), mbar_init(qfull, 256);
-        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 8), mbar_init(gempty(s), MN_LOADERS + 256);
+        mbar_init(oempty, 8), mbar_init(qfull, 8);
+        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 1), mbar_init(gempty(s), 1 + 8);
+        for (int s = 0; s < MN_AHEAD; s++) mbar_init(rfull(s), 1), mbar_init(rempty(s), MN_LOADERS / 32);
         abort_flag = 0;
         mbar_init_fence();
     }
@@ -225,52 +243,36 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     unsigned int *err = a.err;
     const uint32_t smb = smem_u32(sm);
 
+    // pieces in the order K0, K1, V0, K2, V1, ..., V(nt - 1)
+    const int np = 2 * nt;
+    auto tile_of = [&](int i) { return i == 0 ? 0 : i == np - 1 ? nt - 1 : (i & 1) ? (i + 1) / 2 : i / 2 - 1; };
+    auto is_v = [&](int i) { return i == np - 1 || (i != 0 && (i & 1) == 0); };
+    // one arrival for the warp, after what all its lanes have done
+    auto warp_arrive = [&](uint32_t bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+
     if (warp < MN_LOADERS / 32) {
         // ------------------------------ loaders ------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        // pieces in the order K0, K1, V0, K2, V1, ..., V(nt - 1); 16-byte units, TPR threads a row
+        // 16-byte units, TPR threads a row
         constexpr int TPR = HD == 96 ? 8 : HD / 16, RP = MN_LOADERS / TPR, NP = 128 / RP;   // rows a pass, passes
-        static_assert(RP % 16 == 0 && NP >= 1, "whole groups of 16 tokens a pass");
         const int c = tid % TPR, tr = tid / TPR;
         const bool on = c < HD / 16;
-        const uint32_t raw = smb + M::RAW + tid * 16;
-        const int np = 2 * nt;
-        auto tile_of = [&](int i) { return i == 0 ? 0 : i == np - 1 ? nt - 1 : (i & 1) ? (i + 1) / 2 : i / 2 - 1; };
-        auto is_v = [&](int i) { return i == np - 1 || (i != 0 && (i & 1) == 0); };
-        auto load = [&](int i) -> bool {
-            if (i < np) {
-                const int j = tile_of(i), e = j % MN_PAGES;
-                const bool isv = is_v(i);
-                if (!mn_wait(gfull(e), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA)) return false;
-                const uint8_t *base = (const uint8_t *)(isv ? a.kv.v : a.kv.k);
-                const uint8_t *src = base + (tr & 15) * HD + c * 16;
-                const uint32_t dst = raw + (i % MN_AHEAD) * M::PIECE;
-                const int live = kvlen - (p0 + 128 * j);
-                if (on) {
-#pragma unroll
-                    for (int k = 0; k < NP; k++) {
-                        const long long at = page_at[e][k * (RP / 16) + (tr >> 4)];
-                        const bool have = at >= 0 && k * RP + tr < live;
-                        cp_async_zfill<16>(dst + k * (MN_LOADERS * 16), have ? src + at : base, have);
-                    }
-                }
-                if (isv) mbar_arrive(gempty(e));
-            }
-            cp_commit();
-            return true;
-        };
         bool ok = true;
-        for (int i = 0; i < MN_AHEAD && ok; i++) ok = load(i);
 #pragma unroll 1
         for (int i = 0; i < np && ok; i++) {
-            const int j = tile_of(i), s = j & 1;
+            const int j = tile_of(i), s = j & 1, slot = i % MN_AHEAD;
             const bool isv = is_v(i);
-            cp_wait<MN_AHEAD - 1>();
-            if (j >= 2) ok = mn_wait(isv ? ofull(s) : sfull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-            if (isv && j == 0) ok = mn_wait(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);   // V's space held the queries
+            ok = mn_wait(rfull(slot), (i / MN_AHEAD) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+            if (ok && j >= 2) ok = mn_wait(isv ? ofull(s) : sfull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            if (ok && isv && j == 0) ok = mn_wait(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);   // V's space held the queries
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            const int live = kvlen - (p0 + 128 * j);   // rows behind the request's last token count as zeros
             unsigned char *dst = sm + (isv ? M::V : M::K) + s * M::TILE + 2 * c * MN_CHUNK + tr * 16;
-            const unsigned char *src = sm + M::RAW + tid * 16 + (i % MN_AHEAD) * M::PIECE;
+            const unsigned char *src = sm + M::RAW + slot * M::PIECE + tr * HD + c * 16;
             // of its two chunks a thread stores the second one first if c & 4: eight threads of a row
             // then store into different banks
             const bool swap = (c & 4) != 0;
@@ -278,7 +280,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             if (on) {
 #pragma unroll
                 for (int k = 0; k < NP; k++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(src + k * (MN_LOADERS * 16));
+                    uint4 w = *reinterpret_cast<const uint4 *>(src + k * (RP * HD));
+                    if (live < 128 && k * RP + tr >= live) w = make_uint4(0, 0, 0, 0);
                     uint4 h0, h1;
                     codes_h2<TYPE>(swap ? w.z : w.x, h0.x, h0.y);
                     codes_h2<TYPE>(swap ? w.w : w.y, h0.z, h0.w);
@@ -289,10 +292,12 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 }
             }
             fence_proxy_async();
-            mbar_arrive(isv ? vfull(s) : kfull(s));
-            ok = load(i + MN_AHEAD);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(isv ? vfull(s) : kfull(s));
+                mbar_arrive(rempty(slot));
+            }
         }
-        cp_wait<0>();
         __syncwarp();
         mn_roles_done();
         asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(qfull);
+            warp_arrive(qfull);
         }
         float m = -INFINITY, mv = -INFINITY, l = 0.0f;
         float acc[HC];
@@ -374,8 +379,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         const int lim = pos + min(q, nq - 1) / G;
         // adds O of tile j to the registers
         auto drain = [&](int j) -> bool {
-            const bool ok = mn_wait(ofull(j & 1), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-            if (!__all_sync(0xffffffffu, ok)) return false;
+            const bool there = mn_wait(ofull(j & 1), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+            if (!__all_sync(0xffffffffu, there)) return false;
             tc_fence_after();
             uint32_t v[HC];
 #pragma unroll
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             for (int d = 0; d < HC; d += 2)
                 unf2(add2(f2(acc[d], acc[d + 1]), f2(__uint_as_float(v[d]), __uint_as_float(v[d + 1]))), acc[d], acc[d + 1]);
             tc_fence_before();
-            mbar_arrive(oempty);
+            warp_arrive(oempty);
             return true;
         };
         bool ok = true;
@@ -402,11 +407,11 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             tc_fence_after();
             uint32_t v[16 * NG];
             float mx = -INFINITY, mxv = -INFINITY, shrink = 1.0f;
-            if (NG == 1) {
+            if constexpr (NG == 1) {
                 tmem_ld16(t_g, v);
             } else {
                 tmem_ld32(t_g, v);
-                if (NG == 4) tmem_ld32(t_g + 32, v + 16 * (NG - 2));
+                if constexpr (NG == 4) tmem_ld32(t_g + 32, v + 32);
             }
             const int t0 = p0 + 128 * j + 16 * g0;
             float fk[NG];
@@ -496,15 +501,17 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(pfull(b));
-            mbar_arrive(gempty(e));
+            warp_arrive(pfull(b));
+            if (lane == 0) {
+                mbar_arrive(gempty(e));
+            }
             if (j > 0) ok = drain(j - 1);
             if (__any_sync(0xffffffffu, shrink != 1.0f)) {
 #pragma unroll
                 for (int d = 0; d < HC; d++) acc[d] *= shrink;
             }
         }
-        if (ok && nt > 0) drain(nt - 1);
+        if (ok && nt > 0) ok = drain(nt - 1);
         // outputs in units of 2^m
         red[0][half][row].x = l;
         ok = bar_and(1, 256, ok);
@@ -561,49 +568,56 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         mn_roles_done();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        if (warp == 16 && lane == 0) {
+        if (warp == 16) {
             // ------------------------------ S = Q K^T ------------------------------
             const uint32_t idesc = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-            bool go = nt > 0 && mn_wait(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);
+            bool ok = nt > 0 && mbar_wait_warp(qfull, 0, abortp, err, VXC_DERR_TIMEOUT_EPI);
 #pragma unroll 1
-            for (int j = 0; j < nt && go; j++) {
+            for (int j = 0; j < nt && ok; j++) {
                 const int s = j & 1;
-                bool ok = mn_wait(kfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+                ok = mbar_wait_warp(kfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
                 // the buffer's weights (tile j - 2) have been multiplied
-                if (ok && j >= 2) ok = mn_wait(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                if (ok && j >= 2) ok = mbar_wait_warp(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t kd = sdesc(smb + M::K + s * M::TILE, MN_CHUNK, 128);
                 const uint32_t d = tmem + 128 * s;
+                if (mn_elect()) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
-                    const uint64_t bd = kd + (uint64_t)((k * 2 * MN_CHUNK) >> 4);
-                    mma_f16_ts(d, t_q + 8 * k, bd, idesc, k != 0);
-                    mma_f16_ts(d, t_q + 64 + 8 * k, bd, idesc, 1u);
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint64_t bd = kd + (uint64_t)((k * 2 * MN_CHUNK) >> 4);
+                        mma_f16_ts(d, t_q + 8 * k, bd, idesc, k != 0);
+                        mma_f16_ts(d, t_q + 64 + 8 * k, bd, idesc, 1u);
+                    }
+                    mma_commit(sfull(s));
                 }
-                mma_commit(sfull(s));
+                __syncwarp();
             }
-        } else if (warp == 17 && lane == 0) {
+        } else if (warp == 17) {
             // ------------------------------ O = P V ------------------------------
             // V is MN-major (bit 16): 8-column chunks MN_CHUNK apart, groups of 8 tokens 128 bytes apart
             const uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            bool ok = true;
 #pragma unroll 1
-            for (int j = 0; j < nt; j++) {
+            for (int j = 0; j < nt && ok; j++) {
                 const int s = j & 1;
-                bool ok = mn_wait(vfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
-                ok = ok && mn_wait(pfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
-                if (ok && j >= 1) ok = mn_wait(oempty, (j - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                ok = mbar_wait_warp(vfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+                ok = ok && mbar_wait_warp(pfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                if (ok && j >= 1) ok = mbar_wait_warp(oempty, (j - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t vd = sdesc(smb + M::V + s * M::TILE, 128, MN_CHUNK);
                 const uint32_t p = tmem + 128 * s;
+                if (mn_elect()) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const uint64_t bd = vd + (uint64_t)((k * 256) >> 4);
-                    mma_f16_ts(t_o, p + 16 * k, bd, idesc, k != 0);
-                    mma_f16_ts(t_o, p + 16 * k + 8, bd, idesc, 1u);
+                    for (int k = 0; k < 8; k++) {
+                        const uint64_t bd = vd + (uint64_t)((k * 256) >> 4);
+                        mma_f16_ts(t_o, p + 16 * k, bd, idesc, k != 0);
+                        mma_f16_ts(t_o, p + 16 * k + 8, bd, idesc, 1u);
+                    }
+                    mma_commit(ofull(s));
                 }
-                mma_commit(ofull(s));
+                __syncwarp();
             }
         } else if (warp == 18) {
             // ------------------------------ blocks and scales ------------------------------
@@ -637,9 +651,46 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                         page_ks[e][lane & 7] = ks;
                         page_vs[e][lane & 7] = vs;
                         page_lv[e][lane & 7] = lv;
-                        mbar_arrive(gfull(e));
                     }
+                    warp_arrive(gfull(e));
                 }
+            }
+        } else if (warp == 19) {
+            // ------------------------------ copies ------------------------------
+            // a group of 16 tokens is one span of its block: lane = group; groups without a block are zeros
+            bool ok = true;
+            int i = 0;
+#pragma unroll 1
+            for (; i < np; i++) {
+                const int j = tile_of(i), e = j % MN_PAGES, slot = i % MN_AHEAD;
+                const bool isv = is_v(i);
+                ok = mn_wait(gfull(e), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
+                if (ok && i >= MN_AHEAD) ok = mn_wait(rempty(slot), ((i / MN_AHEAD) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const long long at = lane < 8 ? page_at[e][lane] : -1;
+                const unsigned have = __ballot_sync(0xffffffffu, at >= 0), none = ~have & 0xFFu;
+                unsigned char *raw = sm + M::RAW + slot * M::PIECE;
+                if (none) {
+                    for (int g = 0; g < 8; g++)
+                        if ((none >> g) & 1u)
+                            for (int u = lane; u < HD; u += 32)
+                                *reinterpret_cast<uint4 *>(raw + g * 16 * HD + u * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();   // the next piece in this place comes by the asynchronous proxy
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_expect_tx(rfull(slot), __popc(have) * 16 * HD);
+                    if (isv) mbar_arrive(gempty(e));
+                }
+                __syncwarp();
+                if (at >= 0)
+                    bulk_g2s(smem_u32(raw) + lane * 16 * HD, (const uint8_t *)(isv ? a.kv.v : a.kv.k) + at, 16 * HD, rfull(slot));
+            }
+            // after an abort: the pieces on their way land first (bounded)
+            for (int k = i > MN_AHEAD ? i - MN_AHEAD : 0; k < i; k++) {
+                const uint64_t t1 = vxc_globaltimer();
+                while (!mbar_try(rfull(k % MN_AHEAD), (k / MN_AHEAD) & 1) && vxc_globaltimer() - t1 < 100000000ull) {}
             }
         }
         __syncwarp();
@@ -648,7 +699,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     }
 
     // ------------------------------ end ------------------------------
-    if ((warp == 16 || warp == 17) && lane == 0 && *abortp) {
+    if ((warp == 16 || warp == 17) && __any_sync(0xffffffffu, *abortp != 0) && mn_elect()) {
         // an aborted issuer's products may still run: wait for them (bounded)
         const uint32_t bar = bar0 + 8u * (warp == 16 ? 16 : 17);
         mma_commit(bar);
