@@ -88,7 +88,8 @@ cudaError_t kv8_allow_smem(const void *kernel, size_t bytes) {
 //    the request held the block before the call, else the ring entry it takes
 //    (another CTA may not have written the table yet).
 // Bound by latency: one pass over the lengths, a scan, one dependent load and
-// a store per row.
+// a store per row.  Measured: 8 requests of one new token 4.5 us, 250 5.0 us;
+// 32 prompts, 98 thousand rows, 12 us.
 #define TB_THREADS 1024
 #define TB_CLUSTER 8
 #define TB_CLUSTER_ROWS 8192   // rows from which a cluster of TB_CLUSTER CTAs is used
@@ -320,7 +321,9 @@ int vxc_kv8_tables_only(const int *d_len, const int *d_new, int n_req, int block
 // rows are AP_HELD passes, and the window so that a team has about one run: a
 // CTA that finds no run costs a slot on its SM for the time of a load (with
 // windows of 16 rows and blocks of 64 these took longer than the work).
-// Bytes bound it: 4 read and 1 written per element.
+// Bytes bound it: 4 read and 1 written per element.  Measured (heads of 128): 50
+// thousand rows of 8 kv heads 100 us, 5.1 TB/s (windows of 16 rows and one team
+// a CTA: 319 us); 32 requests of 7 rows 5.9 us; 8 rows of 32 kv heads 4.4 us.
 #define AP_THREADS 256
 #define AP_HELD 8
 

@@ -11,8 +11,9 @@ namespace cg = cooperative_groups;
 // Few queries per kv head (decode and small verify steps): split over the
 // context, warp-level tensor instructions.
 //
-// CTA = (request, kv head) x one split of the request's tokens.  Queries are the request's rows times the heads of the kv head,
-// query = row * G + head, so every byte of the split is read once for all.
+// CTA = (request, kv head) x one split of the request's tokens.  Queries are
+// the request's rows times the heads of the kv head, query = row * G + head, so
+// every byte of the split is read once for all.
 // Each of the 4 warps goes over every fourth piece of 32 tokens (two tiles of
 // 16), with a softmax state and an output of its own; the warps are joined at
 // the end.
@@ -44,6 +45,12 @@ namespace cg = cooperative_groups;
 // Tokens behind the request's last one and blocks outside the cache are read
 // as zeros (cp.async's zero fill), so nothing of theirs reaches a product.
 // The blocks and scales of the split are looked up once, at the start.
+//
+// Measured (heads of 128): 33 requests of one row behind up to 16384 tokens, 64
+// heads over 8, 100 us, 5.4 TB/s of the cache's bytes; 8 requests of 5 rows
+// behind up to 768 tokens, 32 heads, 13.6 us; 8 of one row, 32 heads of 64 over
+// 4, 7.4 us.  Bound: bytes for long contexts (issue slots 40 %, tensor pipe
+// 33 % busy); a CTA's latencies, about 4 us, for short ones.
 // ---------------------------------------------------------------------------
 #define FEW_STAGES 2     // 32-token pieces per warp: one in use, one in flight (3: no faster, 4: fewer CTAs per SM, slower)
 
