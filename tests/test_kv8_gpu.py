@@ -173,10 +173,17 @@ def test_attn_context_of_over_half_a_million_tokens(cuda):
 def test_attn_many_requests(cuda):
     rng = np.random.default_rng(3)
     check_attn(cuda, INT8, 64, 2, 2, 16, rng.integers(0, 70, 300).tolist(), rng.integers(0, 3, 300).tolist())
-    # begun by length: equal ones, 128 and one more
-    for n, new in ((128, 1), (129, 1), (128, 20), (129, 20), (5, 9)):
-        check_attn(cuda, INT8, 32, 4, 3, 16, rng.integers(0, 4, n).tolist(), [new] * n)
-    check_attn(cuda, INT8, 32, 40, 3, 16, [7] * 9, [9] * 9)
+    # begun by length: equal ones and a long one, 128 requests and one more
+    for n, kh, new in ((128, 4, 1), (129, 4, 1), (80, 4, 20), (129, 4, 20), (5, 80, 1), (5, 60, 9)):
+        lens = rng.integers(0, 4, n)
+        lens[n // 2] = 600
+        check_attn(cuda, INT8, 32, kh, 3, 16, lens.tolist(), [new] * n)
+    # prompts of few tokens: their queries in pieces of 16
+    for kind, hd, g, most in ((INT8, 32, 1, 26), (E4M3, 64, 3, 40), (INT8, 32, 5, 30), (E4M3, 32, 16, 9)):
+        new = rng.integers(0, most + 1, 90)
+        new[0] = most
+        check_attn(cuda, kind, hd, 24, g, 16, rng.integers(0, 20, 90).tolist(), new.tolist())
+        check_attn(cuda, kind, hd, 24, g, 16, rng.integers(-9, 3, 90).tolist(), np.maximum(new, 10).tolist())
 
 
 def test_attn_requests_without_rows_and_rows_without_tokens(cuda):

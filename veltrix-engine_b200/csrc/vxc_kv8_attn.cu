@@ -96,15 +96,17 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     pdl_trigger();
     pdl_wait();
     // (scratch in the ring: static shared memory would move the ring off its 128-byte lines, +6 %)
-    const int r = a.ranked ? kv8_ranked<128>(a, blockIdx.z, reinterpret_cast<int *>(sm)) : blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    const int kvh = blockIdx.y, split = blockIdx.x, place = (int)blockIdx.z / a.chunks;
+    const int q0 = ((int)blockIdx.z - place * a.chunks) * NQ;   // first query of the CTA
+    const int r = a.ranked ? kv8_ranked(a, place, reinterpret_cast<int *>(sm)) : place;
     const Kv8Req rq = kv8_req(a, r);
-    if (rq.over && kvh == 0 && split == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
-    const int nq = rq.T * G;   // at most NQ
-    if (nq == 0) return;
+    if (rq.over && kvh == 0 && split == 0 && q0 == 0 && tid == 0) vxc_flag_error(a.err, VXC_DERR_BAD_BLOCK);
+    const int nq = min(rq.T * G - q0, NQ);
+    if (nq <= 0) return;
     int SL;
     const int ns = kv8_splits(rq.kvlen, a.sl_min, a.S, SL);
     if (split >= ns) return;
-    const int p0 = split * SL, p1 = min(p0 + SL, rq.kvlen);
+    const int p0 = split * SL, p1 = min(p0 + SL, rq.pos + (q0 + nq - 1) / G + 1);
 
     // blocks (-1: outside the cache) of the split, then their {K scale, V scale, its logarithm}
     const int e0 = p0 / bs, ne = p1 > p0 ? (p1 - 1) / bs - e0 + 1 : 0;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     for (int i = 0; i < NR; i++) {
         const int q = g + 8 * i;
         const bool have = q < nq;
-        const int row = rq.row0 + (have ? q / G : 0), h = kvh * G + (have ? q % G : 0);
+        const int row = rq.row0 + (have ? (q0 + q) / G : 0), h = kvh * G + (have ? (q0 + q) % G : 0);
         const float *x = a.q + (size_t)row * a.ldq + (size_t)h * HD;
         float4 v[KS];
         float mx = 0.0f;
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         const int ex = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
         const float up = __uint_as_float((uint32_t)(267 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 13) << 23);
         f[i] = a.scale * 1.4426950408889634f * down;
-        lim[i] = have ? rq.pos + q / G : -1;
+        lim[i] = have ? rq.pos + (q0 + q) / G : -1;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             uint32_t l0, l1;
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
             mw[k] = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
             L += mw[k] * sml[(k * NQ + q) * 2 + 1];
         }
-        const int row = rq.row0 + q / G, h = kvh * G + q % G;
+        const int row = rq.row0 + (q0 + q) / G, h = kvh * G + (q0 + q) % G;
         float *rec = cluster ? res + q * (HD + 4) : a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
         float *out = a.out + (size_t)row * a.ldo + (size_t)h * HD;
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
@@ -529,6 +531,7 @@ static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int
 // How a call is cut: kernel, queries per CTA and splits.
 struct AttnPlan {
     int nq;        // queries per CTA: 8 or 16 (k_kv8_attn_few), 32, 64 or 128 (k_kv8_attn_many)
+    int chunks;    // k_kv8_attn_few: CTAs for a request's queries
     int tiles;     // k_kv8_attn_many: tiles of all requests at most
     int S, sl_min;
     int pages;     // blocks a split may touch (k_kv8_attn_few)
@@ -539,6 +542,7 @@ struct AttnPlan {
 
 static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
     AttnPlan p;
+    p.chunks = 1;
     const int G = n_heads / kv->n_kv_heads;
     const long long most = (long long)(max_new < n_rows ? max_new : n_rows) * G;   // queries of a request
     const long long tokens = (long long)max_blocks * kv->block_size;
@@ -587,6 +591,20 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
             const double join = i == 1 ? 0 : 3 + 2e-6 * n_rows * n_heads * i * (kv->head_dim + 4);
             const double time = (cta > all ? cta : all) + join;
             if (i == 1 || time < best) best = time, S = i;
+        }
+        // Many requests of few tokens: k_kv8_attn_few's CTAs, of 16 queries each, cost less (6.5 us besides
+        // their tokens in a queue of them; 2 fit an SM, 3 with heads of 64, 4 with heads of 32).  100 requests
+        // of 26 rows in 26 tokens, 28 heads of 32: 389 us in tiles, 46 so.  Where the estimates are near each
+        // other the tile is kept: 43 requests of 16 rows in 51 tokens, 30 heads of 128 over 10, 32 and 33 us.
+        const long long chunks = (most + 15) / 16;
+        const double byte = kv->head_dim / 128.0, cta = 4 + 0.0125 * byte * tokens;
+        const int places = 148 * (kv->head_dim >= 96 ? 2 : kv->head_dim == 64 ? 3 : 4);
+        const double all = (double)n_req * kv->n_kv_heads * chunks * (6.5 + 0.75 * 0.0144 * byte * tokens) / places + 0.25 * cta;
+        if (tokens <= 8192 && chunks * n_req <= 65535 && (cta > all ? cta : all) < 0.7 * best) {
+            p.nq = 16;
+            p.chunks = (int)chunks;
+            p.sl_min = (int)((tokens + 127) & ~127ll);
+            S = 1;
         }
     }
     const long long need = (tokens + p.sl_min - 1) / p.sl_min;
@@ -642,11 +660,14 @@ static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st)
     Kv8AttnArgs a = args;
     a.S = p.S;
     a.sl_min = p.sl_min;
+    a.chunks = p.chunks;
     a.pages = p.pages;
-    // (where all CTAs fit the GPU at once, one or two per SM, the order is of no use)
+    // the order is of no use where all CTAs fit the GPU at once, one or two per SM; its cost, a load and
+    // n_req comparisons per CTA, is more than it gives where there are many more or contexts are short
     const bool many = p.nq > ATTN_FEW_MAX;
-    a.ranked = (!many || p.tiles == a.n_req) && a.n_req > 1 && a.n_req <= KV8_RANKED &&
-               (long long)a.n_req * a.kv.n_kv_heads * p.S > (many ? 148 : 2 * 148);
+    const long long ctas = (long long)a.n_req * a.kv.n_kv_heads * p.S * p.chunks, at_once = many ? 148 : 2 * 148;
+    a.ranked = (!many || p.tiles == a.n_req) && a.n_req > 1 && a.n_req <= KV8_RANKED && ctas > at_once && ctas <= 4 * at_once &&
+               (long long)a.max_blocks * a.kv.block_size > 512;
     a.err = vxc_device_error_ptr();
     const vxc_kv8 *kv = &a.kv;
     const int hd = kv->head_dim;
@@ -658,7 +679,7 @@ static int attn_run(const Kv8AttnArgs &args, const AttnPlan &p, cudaStream_t st)
         const size_t join = ((size_t)4 * p.nq * (hd + 6) + (size_t)p.nq * (hd + 4)) * sizeof(float);
         if (smem < join) smem = join;
         VXC_CUDA_OK(kv8_allow_smem((const void *)f, smem));
-        VXC_CUDA_OK(kv8_launch(f, dim3(p.S, kv->n_kv_heads, a.n_req), dim3(128), smem, st,
+        VXC_CUDA_OK(kv8_launch(f, dim3(p.S, kv->n_kv_heads, a.n_req * p.chunks), dim3(128), smem, st,
                                p.S <= 8 ? p.S : 1, a));
     }
     if (attn_records(p))

@@ -22,6 +22,7 @@ struct Kv8AttnArgs {
     float *part;        // records of the splits
     int S, sl_min;      // splits per request at most, tokens per split at least
     int pages;          // blocks a split may touch, rounded up to 4 (k_kv8_attn_few)
+    int chunks;         // k_kv8_attn_few: CTAs with their own queries per request, kv head and split (then S is 1)
     int ranked;         // requests begin by length, longest first (at most KV8_RANKED)
     unsigned int *err;
 };
@@ -124,37 +125,23 @@ __device__ __forceinline__ Kv8Req kv8_req(const Kv8AttnArgs &a, int r) {
 // (33 requests of one row behind up to 16384 tokens: 124 -> 100 us; 32 of 7 rows behind up to 4096:
 // 122 -> 112 us.)  The position is length enough.
 #define KV8_RANKED 128
-// The request whose position is the k-th largest.  Called by THREADS threads, one warp or a whole block;
-// pos_s: KV8_RANKED + 1 ints of shared memory, 16-byte aligned.
-template <int THREADS>
+// The request whose position is the k-th largest.  Called by the block's first KV8_RANKED threads (one
+// warp with four requests a lane took 4 us for 43 of them); pos_s: KV8_RANKED + 1 ints of shared memory,
+// 16-byte aligned.
 __device__ __forceinline__ int kv8_ranked(const Kv8AttnArgs &a, int k, int *pos_s) {
-    constexpr int KEYS = KV8_RANKED / THREADS;
-    auto sync = [] {
-        if (THREADS == 32) __syncwarp();
-        else __syncthreads();
-    };
-    const int me = threadIdx.x % THREADS, n = a.n_req;
-    int key[KEYS], rank[KEYS];
-#pragma unroll
-    for (int i = 0; i < KEYS; i++) {
-        const int r = me + THREADS * i;
-        key[i] = r < n ? a.pos[r] : INT_MIN;
-        rank[i] = 0;
-        pos_s[r] = key[i];
-    }
+    auto sync = [] { asm volatile("bar.sync 3, %0;" ::"n"(KV8_RANKED) : "memory"); };
+    const int me = threadIdx.x, n = a.n_req, key = me < n ? a.pos[me] : INT_MIN;
+    pos_s[me] = key;
     sync();
-    for (int o = 0; o < n; o += 4) {   // (INT_MIN behind the last: counts for no request)
-        const int4 p = *reinterpret_cast<const int4 *>(pos_s + o);
-#pragma unroll
-        for (int i = 0; i < KEYS; i++) {
-            const int r = me + THREADS * i;
-            auto count = [&](int x, int at) { rank[i] += x > key[i] || (x == key[i] && at < r); };
-            if (i == 0 || THREADS * i < n) count(p.x, o), count(p.y, o + 1), count(p.z, o + 2), count(p.w, o + 3);
+    if (me < n) {
+        int rank = 0;
+        auto count = [&](int p, int o) { rank += p > key || (p == key && o < me); };
+        for (int o = 0; o < n; o += 4) {   // (INT_MIN behind the last: counts for no request)
+            const int4 p = *reinterpret_cast<const int4 *>(pos_s + o);
+            count(p.x, o), count(p.y, o + 1), count(p.z, o + 2), count(p.w, o + 3);
         }
+        if (rank == k) pos_s[KV8_RANKED] = me;
     }
-#pragma unroll
-    for (int i = 0; i < KEYS; i++)
-        if (me + THREADS * i < n && rank[i] == k) pos_s[KV8_RANKED] = me + THREADS * i;
     sync();
     return pos_s[KV8_RANKED];
 }

@@ -184,12 +184,14 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     }
     if (warp == 16) tmem_alloc(smem_u32(&tmem_slot), 512u);
     pdl_wait();
+    int nth = tiles - 1 - tile;
+    if (a.ranked && tid < KV8_RANKED) nth = kv8_ranked(a, tile, reinterpret_cast<int *>(sm));
     if (warp == 0) {
         // request and query tile: tiles of request r begin at floor(row0 G / TQ) + r, which leaves
         // every request as many as it needs; later tiles (longer contexts) first.  (One warp: the
         // same work by all of them took 2000 cycles more.)
         const bool one = tiles == a.n_req;   // a tile per request
-        const int idx = a.ranked ? kv8_ranked<32>(a, tile, reinterpret_cast<int *>(sm)) : tiles - 1 - tile;
+        const int idx = nth;
         int r = one ? idx : 0, len = one ? 1 : a.n_req, r0, r1, pos, seq;
         do {   // 32 places a step
             const int step = (len + 31) / 32, at = lane * step, ri = r + at;
