@@ -144,3 +144,11 @@ def test_groups_outside_the_set_are_reported(cuda):
     assert rc == -4 and b"one group per slot" in s.L.vxc_error_string()
     assert s.forward(ids[1:], [0], [0])[1] == 0
     s.close()
+
+
+def test_contexts_over_the_limit_are_refused(cuda):
+    s = Seqs(cuda, INT8, 1, 64, 64)
+    for max_ctx in ((1 << 30) + 1, 2 ** 31 - 1):
+        h = ctypes.c_void_p()
+        assert s.L.vxc_seqs_create_kv8(s.net, 1, max_ctx, 64, INT8, 64, 4, ctypes.byref(h)) == -4 and not h.value
+    s.close()

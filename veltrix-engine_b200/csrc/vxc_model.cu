@@ -1451,7 +1451,7 @@ static int seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_row
     const int nch = (max_rows + 63) / 64;
     if (kv_type) {
         // as many blocks as every slot's context needs, unless told otherwise
-        const int per = (max_ctx + (block_size > 0 ? block_size : 1) - 1) / (block_size > 0 ? block_size : 1);
+        const int per = (int)(((long long)max_ctx + (block_size > 0 ? block_size : 1) - 1) / (block_size > 0 ? block_size : 1));
         const long long nb = n_blocks > 0 ? n_blocks : (long long)n_slots * per;
         s->kv8 = {kv_type, (int)(nb < INT_MAX ? nb : INT_MAX), block_size, net->KHl, hd, NULL, NULL, NULL, NULL};
         s->max_blocks = per;
@@ -1460,6 +1460,10 @@ static int seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_row
         s->kv8.k_scale = s->kv8.v_scale = (float *)256;
         rc = n_slots > VXC_KV8_MAX_REQ ? -4 : vxc_kv8_check(&s->kv8, "vxc_seqs_create_kv8");
         if (n_slots > VXC_KV8_MAX_REQ) vxc_set_error("vxc_seqs_create_kv8: %d slots (at most %d)", n_slots, VXC_KV8_MAX_REQ);
+        if (rc == 0 && (long long)per * block_size > 1 << 30) {
+            vxc_set_error("vxc_seqs_create_kv8: context %d (at most 2^30)", max_ctx);
+            rc = -4;
+        }
         if (rc) {
             free(s);
             return rc;
@@ -1523,7 +1527,8 @@ static int seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_row
 #undef ALLOC
     if (kv_type) {
         // empty scales and tables, every block free
-        std::vector<int> h(i8, 0);
+        int *h = (int *)calloc(i8, sizeof(int));
+        if (!h && e == cudaSuccess) e = cudaErrorMemoryAllocation;
         s->table = s->i8;
         s->held = s->table + (size_t)n_slots * s->max_blocks;
         s->row0 = s->held + n_slots;
@@ -1533,10 +1538,13 @@ static int seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_row
         s->ring = s->state + 3;
         s->seq = s->ring + s->kv8.n_blocks;
         s->tok_slot = s->seq + max_rows;
-        for (size_t i = 0; i < (size_t)n_slots * s->max_blocks; i++) h[i] = -1;
-        h[s->state - s->i8 + 1] = s->kv8.n_blocks;
-        for (int b = 0; b < s->kv8.n_blocks; b++) h[s->ring - s->i8 + b] = b;
-        if (e == cudaSuccess) e = cudaMemcpy(s->i8, h.data(), i8 * 4, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) {
+            for (size_t i = 0; i < (size_t)n_slots * s->max_blocks; i++) h[i] = -1;
+            h[s->state - s->i8 + 1] = s->kv8.n_blocks;
+            for (int b = 0; b < s->kv8.n_blocks; b++) h[s->ring - s->i8 + b] = b;
+            e = cudaMemcpy(s->i8, h, i8 * 4, cudaMemcpyHostToDevice);
+        }
+        free(h);
         if (e == cudaSuccess) e = cudaMemset(s->kv8.k, 0, b8);
         if (e == cudaSuccess) e = cudaMemset(s->kv8.v, 0, b8);
         if (e == cudaSuccess) e = cudaMemset(s->kv8.k_scale, 0, n8 * 4);
