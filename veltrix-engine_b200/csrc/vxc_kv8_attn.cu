@@ -551,9 +551,9 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         p.nq = most <= 8 ? 8 : 16;
         p.tiles = 0;
         units = (long long)n_req * kv->n_kv_heads;
-        // A CTA costs about 4 us besides its tokens and, joined by a cluster, 2 us more; two fit an SM, and
-        // each further CTA of a unit takes 12 us of a place (a cluster's CTAs begin and end together); above
-        // 8 a second kernel joins them.  The S of the least time, as below; measured (us, S = 1, 2, ...):
+        // A CTA costs about 4 us besides its tokens and, joined by a cluster, 2 us more; two fit an SM, a
+        // cluster's on one of 8 groups of 16 SMs or more, and each further CTA of a unit takes 12 us of a place
+        // (a cluster's CTAs begin and end together); above 8 a second kernel joins them.  The S of the least time, as below; measured (us, S = 1, 2, ...):
         // 256 units of 768 tokens 13.5, 17.5; 256 of 4096 58, 47, 53; 512 of 8192 108, 127, 157; 800 of
         // 4096 105, 136, 146; 264 of 16384 -, 105, 120, 138; 32 of 768 9.2, in six 7.3.
         p.sl_min = 128;
@@ -563,9 +563,10 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         for (int i = 1; i <= 64; i++) {
             const double cta = 4 + 0.0125 * byte * tokens / i + (i == 1 ? 0 : i <= 8 ? 2 : 8);
             const double places = i <= 8 ? 4 + 12.0 * (i - 1) : 6.0 * i;
-            const double all = n_req == 1 ? (units * i + 295) / 296 * cta
+            const long long room = i == 1 || i > 8 ? 296 / i : 8 * (32 / i);   // units that fit at once
+            const double all = n_req == 1 ? (units + room - 1) / room * cta
                                           : units * (places + 0.5 * 0.0144 * byte * tokens) / 296 + 0.25 * cta;
-            const double time = cta > all || units * i <= 296 ? cta : all;
+            const double time = cta > all || units <= room ? cta : all;
             if (i == 1 || time < best) best = time, S = i;
         }
     } else {
@@ -600,7 +601,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         const double byte = kv->head_dim / 128.0, cta = 4 + 0.0125 * byte * tokens;
         const int places = 148 * (kv->head_dim >= 96 ? 2 : kv->head_dim == 64 ? 3 : 4);
         const double all = (double)n_req * kv->n_kv_heads * chunks * (6.5 + 0.75 * 0.0144 * byte * tokens) / places + 0.25 * cta;
-        if (tokens <= 8192 && chunks * n_req <= 65535 && (cta > all ? cta : all) < 0.7 * best) {
+        if (tokens <= 8192 && chunks * n_req <= 65535 && (cta > all ? cta : all) < 0.8 * best) {
             p.nq = 16;
             p.chunks = (int)chunks;
             p.sl_min = (int)((tokens + 127) & ~127ll);
