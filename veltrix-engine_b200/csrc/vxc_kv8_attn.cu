@@ -553,9 +553,10 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         units = (long long)n_req * kv->n_kv_heads;
         // A CTA costs about 4 us besides its tokens and, joined by a cluster, 2 us more; two fit an SM, a
         // cluster's on one of 8 groups of 16 SMs or more, and each further CTA of a unit takes 12 us of a place
-        // (a cluster's CTAs begin and end together); above 8 a second kernel joins them.  The S of the least time, as below; measured (us, S = 1, 2, ...):
-        // 256 units of 768 tokens 13.5, 17.5; 256 of 4096 58, 47, 53; 512 of 8192 108, 127, 157; 800 of
-        // 4096 105, 136, 146; 264 of 16384 -, 105, 120, 138; 32 of 768 9.2, in six 7.3.
+        // (a cluster's CTAs begin and end together); above 8 a second kernel joins them.  The S of the least
+        // time, as below; measured (us, S = 1, 2, ...): 256 units of 768 tokens 13.5, 17.5; 256 of 4096 58, 47,
+        // 53; 512 of 8192 108, 127, 157; 800 of 4096 105, 136, 146; 264 of 16384 -, 105, 120, 138; 32 of 768
+        // 9.2, in six 7.3; 48 of 2000 in five 12.8, in six 18.5 (not all of those clusters fit at once).
         p.sl_min = 128;
         double best = 0;
         const double byte = kv->head_dim / 128.0;

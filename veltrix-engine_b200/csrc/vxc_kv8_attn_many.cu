@@ -2,9 +2,9 @@
 // queries per kv head (prompt pieces, wide verify steps) on tcgen05
 // (reference src/model.c:299-338, over its fp32 cache).
 //
-// CTA = (tile of 128 queries of one request and kv head) x one split of its
-// tokens; queries are row * G + head, so a tile is 128 / G consecutive rows and
-// its causal bound is tight.  Tokens go by in tiles of 128:
+// CTA = (tile of 128, 64 or 32 queries of one request and kv head) x one split
+// of its tokens; queries are row * G + head, so a tile is 128 / G consecutive
+// rows and its causal bound is tight.  Tokens go by in tiles of 128:
 //   S = Q K^T    two products per step of 16, Q_hi and Q_lo (from TMEM)
 //   P            softmax weights in place of S in TMEM, hi and lo fp16
 //   O = P V      two products per step
