@@ -37,9 +37,9 @@
 // outputs go as whole rows, through V's slots before and after their use.
 //
 // Measured (heads of 128): 4096 rows behind 12288 tokens, 64 heads over 8,
-// 3.35 ms: 575 Tflop/s of attention, 1.15 Pflop/s of fp16 products, 0.69 of a
+// 3.39 ms: 568 Tflop/s of attention, 1.14 Pflop/s of fp16 products, 0.68 of a
 // library's bf16 product.  8 prompts of up to 512 rows, 32 heads, 97 us; 32
-// requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 87 us.  Bound:
+// requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 86 us.  Bound:
 // a tile takes 3700 cycles, of which 2048 are products.  The softmax warps'
 // chain is as long: waiting for and reading S 900, maxima 400, weights 1800 (64
 // of each thread's exponentials and conversions share a unit of 16 lanes), O
@@ -142,7 +142,7 @@ template <int TYPE, int HD, int TQ>
 __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnArgs a) {
     using M = MnSmem<HD>;
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ __align__(8) uint64_t bars[18 + 2 * MN_PAGES + MN_AHEAD];
+    __shared__ __align__(8) uint64_t bars[18 + 3 * MN_PAGES + MN_AHEAD];
     __shared__ long long page_at[MN_PAGES][8];     // byte offset of a 16-token group in the cache; -1 none, -2 bad block
     __shared__ __align__(16) float page_ks[MN_PAGES][8], page_vs[MN_PAGES][8], page_lv[MN_PAGES][8];
     __shared__ float2 red[2][2][128];              // [tile parity][half][query]: maxima of half a tile
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
     auto pfull = [&](int b) { return bar0 + 8u * (10 + b); };      // its weights stored (softmax warps)
     auto ofull = [&](int b) { return bar0 + 8u * (12 + b); };      // its P V product done: its V slot is free
     const uint32_t oempty = bar0 + 8u * 14, qfull = bar0 + 8u * 15;   // O read; queries stored (softmax warps)
-    auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks and scales of a tile
+    auto gfull = [&](int s) { return bar0 + 8u * (18 + s); };      // blocks of a tile known; its scales
+    auto gscale = [&](int s) { return bar0 + 8u * (18 + 2 * MN_PAGES + MN_AHEAD + s); };
     auto gempty = [&](int s) { return bar0 + 8u * (18 + MN_PAGES + s); };   // the copy warp and the softmax warps are done with them
     auto rempty = [&](int s) { return bar0 + 8u * (18 + 2 * MN_PAGES + s); };   // raw piece read (loader warps)
     static_assert(MN_AHEAD <= 4, "rfull has places 4-7");
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             mbar_init(bar0 + 8u * (16 + s), 1);   // an issuer's last work, after an abort
         }
         mbar_init(oempty, 8), mbar_init(qfull, 8);
-        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 1), mbar_init(gempty(s), 1 + 8);
+        for (int s = 0; s < MN_PAGES; s++) mbar_init(gfull(s), 1), mbar_init(gscale(s), 1), mbar_init(gempty(s), 1 + 8);
         for (int s = 0; s < MN_AHEAD; s++) mbar_init(rfull(s), 1), mbar_init(rempty(s), MN_LOADERS / 32);
         abort_flag = 0;
         mbar_init_fence();
@@ -569,6 +570,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         mn_roles_done();
     } else {
+        int blk0 = -1;   // the page warp's first lookup, on its way early: the first tile waits for it
+        if (warp == 18 && p0 + 16 * lane < kvlen && (lane >> 3) < nt) blk0 = item.table[(p0 + 16 * lane) / bs];
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 16) {
             // ------------------------------ S = Q K^T ------------------------------
@@ -580,6 +583,8 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 ok = mbar_wait_warp(kfull(s), (j >> 1) & 1, abortp, err, VXC_DERR_TIMEOUT_TMA);
                 // the buffer's weights (tile j - 2) have been multiplied
                 if (ok && j >= 2) ok = mbar_wait_warp(ofull(s), ((j >> 1) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_MMA);
+                // (the softmax warps read the scales once S is there)
+                ok = ok && mbar_wait_warp(gscale(j % MN_PAGES), (j / MN_PAGES) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t kd = sdesc(smb + M::K + s * M::TILE, MN_CHUNK, 128);
@@ -631,7 +636,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 long long at = -1;
                 float ks = 0.0f, vs = 0.0f;
                 if (p < kvlen && t + (lane >> 3) < nt) {
-                    const int blk = item.table[p / bs];
+                    const int blk = t == 0 ? blk0 : item.table[p / bs];
                     if (blk >= 0 && blk < a.kv.n_blocks) {
                         const size_t bh = (size_t)blk * KH + kvh;
                         at = (long long)((bh * bs + p % bs) * HD);
@@ -642,19 +647,23 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                         vxc_flag_error(err, VXC_DERR_BAD_BLOCK);
                     }
                 }
-                const float lv = lg2(vs);
                 for (int k = 0; k < 4 && t + k < nt; k++) {
                     const int j = t + k, e = j % MN_PAGES;
                     if (j >= MN_PAGES) ok = mn_wait(gempty(e), ((j / MN_PAGES) - 1) & 1, abortp, err, VXC_DERR_TIMEOUT_EPI);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                    if (lane >> 3 == k) page_at[e][lane & 7] = at;
+                    warp_arrive(gfull(e));
+                }
+                const float lv = lg2(vs);
+                for (int k = 0; k < 4 && t + k < nt && ok; k++) {
+                    const int e = (t + k) % MN_PAGES;
                     if (lane >> 3 == k) {
-                        page_at[e][lane & 7] = at;
                         page_ks[e][lane & 7] = ks;
                         page_vs[e][lane & 7] = vs;
                         page_lv[e][lane & 7] = lv;
                     }
-                    warp_arrive(gfull(e));
+                    warp_arrive(gscale(e));
                 }
             }
         } else if (warp == 19) {
