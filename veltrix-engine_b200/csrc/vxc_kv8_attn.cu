@@ -81,7 +81,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // The splits of a request and head are joined by their cluster, through
 // distributed shared memory, while a cluster holds them all (a.S <= 8); else
 // they leave records in device memory for k_kv8_attn_join:
-// [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, o = sum of 2^(s - m) v.
+// [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, l = sum of 2^(s - m), o = the split's own output.  (Every
+// partial output is divided by its own l and joined with weights 2^(m - M) l / L: sums of
+// 2^(s - m) v themselves would overflow for V within their number of tokens of the largest float.)
 template <int TYPE, int HD, int NQ>
 __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     using P = Kv8Few<HD>;
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     cp_wait<0>();
     __syncthreads();   // the ring is free
 
-    // join the warps: unnormalised outputs in units of 2^m, maxima and sums
+    // join the warps: their outputs, maxima and sums
     float *so = reinterpret_cast<float *>(sm);            // [4][NQ][HD + 4]
     float *sml = so + 4 * NQ * (HD + 4);                  // [4][NQ][2]
 #pragma unroll
@@ -392,13 +394,14 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
         const float back = mv[i] == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv[i] - m[i] - KV8_HEAD, 126.0f), -126.0f));
+        const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];   // no token: 0; NaN stays
         float *dst = so + (w * NQ + g + 8 * i) * (HD + 4);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             const int c = j / P::V, e = j % P::V;
             const float x = NR == 1 ? o[j][0] + o[j][2] : o[j][2 * i], y = NR == 1 ? o[j][1] + o[j][3] : o[j][2 * i + 1];
-            dst[P::v_at(c, 2 * t) + e] = x * back;
-            dst[P::v_at(c, 2 * t + 1) + e] = y * back;
+            dst[P::v_at(c, 2 * t) + e] = x * inv * back;
+            dst[P::v_at(c, 2 * t + 1) + e] = y * inv * back;
         }
         if (t == 0) {
             sml[(w * NQ + g + 8 * i) * 2] = m[i];
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         }
     }
     __syncthreads();
-    // the CTA's result, one warp per query: {m, l, -, -, o[HD]}, unnormalised
+    // the CTA's result, one warp per query: {m, l, -, -, o[HD]}
     const bool cluster = a.S <= 8;
     float *res = sml + 4 * NQ * 2;                        // [NQ][HD + 4]
     for (int q = w; q < nq; q += 4) {
@@ -415,8 +418,8 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         for (int k = 0; k < 4; k++) M = fmaxf(M, mw[k] = sml[(k * NQ + q) * 2]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            mw[k] = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
-            L += mw[k] * sml[(k * NQ + q) * 2 + 1];
+            mw[k] = (mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M)) * sml[(k * NQ + q) * 2 + 1];
+            L += mw[k];
         }
         const int row = rq.row0 + (q0 + q) / G, h = kvh * G + (q0 + q) % G;
         float *rec = cluster ? res + q * (HD + 4) : a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
@@ -427,8 +430,8 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
             float x = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (mw[k] != 0.0f) x = fmaf(mw[k], so[(k * NQ + q) * (HD + 4) + d], x);
-            if (ns == 1) out[d] = x * inv;
+                if (mw[k] != 0.0f) x = fmaf(mw[k] * inv, so[(k * NQ + q) * (HD + 4) + d], x);
+            if (ns == 1) out[d] = x;
             else rec[4 + d] = x;
         }
         if (ns > 1 && lane == 0) *reinterpret_cast<float2 *>(rec) = make_float2(M, L);
@@ -438,26 +441,37 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
     for (int q = split + ns * w; q < nq; q += 4 * ns) {
-        float M = -INFINITY, L = 0.0f, mw[8], x[HD / 32];
+        float M = -INFINITY, L = 0.0f, x[HD / 32];
+        float2 ml[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (k < ns) M = fmaxf(M, mw[k] = *cl.map_shared_rank(res + q * (HD + 4), k));
+        for (int k = 0; k < 8; k++) {
+            if (k < ns) {
+                ml[k] = *reinterpret_cast<const float2 *>(cl.map_shared_rank(res + q * (HD + 4), k));
+                M = fmaxf(M, ml[k].x);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k < ns) {
+                ml[k].y *= ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - M);
+                L += ml[k].y;
+            }
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) x[d] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             if (k < ns) {
                 const float *rec = cl.map_shared_rank(res + q * (HD + 4), k);
-                const float e = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
-                L = fmaf(e, rec[1], L);
+                const float e = ml[k].y * inv;
 #pragma unroll
                 for (int d = 0; d < HD / 32; d++) x[d] = fmaf(e, rec[4 + d * 32 + lane], x[d]);
             }
         }
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         float *out = a.out + (size_t)(rq.row0 + q / G) * a.ldo + (size_t)(kvh * G + q % G) * HD;
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) out[d * 32 + lane] = x[d] * inv;
+        for (int d = 0; d < HD / 32; d++) out[d * 32 + lane] = x[d];
     }
     cl.sync();   // the others have read this CTA's results
 }
@@ -486,17 +500,21 @@ __global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
     const int n = rq.pos + (i - rq.row0) >= 0 ? live : 0;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, rec[(size_t)s * (HD + 4)]);
+    auto head = [&](int s) { return *reinterpret_cast<const float2 *>(rec + (size_t)s * (HD + 4)); };
+    auto unit = [&](float m) { return m == -INFINITY ? 0.0f : ex2(m - M); };   // 2^m in units of 2^M
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, head(s).x);
 #pragma unroll
     for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+    for (int s = lane; s < n; s += 32) L = fmaf(unit(head(s).x), head(s).y, L);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
     // lanes have a record's {m, l} each, then, of one record after the other, four values each
     const float *mine = rec + 4 + 4 * min(lane, HD / 4 - 1);
     for (int at = 0; at < n; at += 32) {
         const int some = min(n - at, 32);
-        const float2 ml = lane < some ? *reinterpret_cast<const float2 *>(rec + (size_t)(at + lane) * (HD + 4))
-                                      : make_float2(-INFINITY, 0.0f);
-        const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        L = fmaf(w, ml.y, L);
+        const float2 ml = lane < some ? head(at + lane) : make_float2(-INFINITY, 0.0f);
+        const float w = unit(ml.x) * ml.y * inv;
 #pragma unroll 8
         for (int s = 0; s < some; s++) {
             const float e = __shfl_sync(0xffffffffu, w, s);
@@ -504,12 +522,7 @@ __global__ void __launch_bounds__(128) k_kv8_attn_join(const Kv8AttnArgs a) {
             if (e != 0.0f) o.x = fmaf(e, x.x, o.x), o.y = fmaf(e, x.y, o.y), o.z = fmaf(e, x.z, o.z), o.w = fmaf(e, x.w, o.w);
         }
     }
-#pragma unroll
-    for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
-    if (lane < HD / 4)
-        *reinterpret_cast<float4 *>(a.out + (size_t)i * a.ldo + (size_t)h * HD + 4 * lane) =
-            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (lane < HD / 4) *reinterpret_cast<float4 *>(a.out + (size_t)i * a.ldo + (size_t)h * HD + 4 * lane) = o;
 }
 
 static int attn_check(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {

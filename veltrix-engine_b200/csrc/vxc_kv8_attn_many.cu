@@ -515,20 +515,19 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             }
         }
         if (ok && nt > 0) ok = drain(nt - 1);
-        // outputs in units of 2^m
         red[0][half][row].x = l;
         ok = bar_and(1, 256, ok);
         if (ok) {
             float L = 0.0f;
 #pragma unroll
             for (int i = 0; i < NP; i++) L += red[0][0][qrow + TQ * i].x + red[0][1][qrow + TQ * i].x;
-            const float inv = ns > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
-            const float back = (mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f))) * inv;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
+            const float back = mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f));
             // (every product has ended: V's space is free)
 #pragma unroll
             for (int d = 0; d < HC; d += 4)
                 *reinterpret_cast<float4 *>(xs + row * XS + half * HC + d) =
-                    make_float4(acc[d] * back, acc[d + 1] * back, acc[d + 2] * back, acc[d + 3] * back);
+                    make_float4(acc[d] * inv * back, acc[d + 1] * inv * back, acc[d + 2] * inv * back, acc[d + 3] * inv * back);
             if (ns > 1 && half == 0 && part == 0 && q < nq) {
                 const int t = q / G, h = kvh * G + q - t * G;
                 *reinterpret_cast<float2 *>(a.part + (((size_t)(row0 + t) * a.H + h) * a.S + split) * (HD + 4)) = make_float2(m, L);
