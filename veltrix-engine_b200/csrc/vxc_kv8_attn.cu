@@ -310,7 +310,9 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
                 m[i] = mm;
             }
             float shrink = 1.0f;
-            if (mxv > mv[i] + KV8_LAG || (mv[i] == -INFINITY && mxv > mv[i])) {
+            const float least = m[i] - KV8_FLOOR;
+            mxv = fmaxf(mxv, least);
+            if (mxv > mv[i] + KV8_LAG || least > mv[i]) {
                 shrink = ex2(mv[i] - mxv);
                 mv[i] = mxv;
             }
@@ -324,15 +326,17 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
                     }
                 }
             }
-            const float mref = m[i] == -INFINITY ? 0.0f : m[i];
-            const float cv = ex2(fminf(mref - mv[i] + KV8_HEAD, 120.0f));
+            float mref = m[i] == -INFINITY ? 0.0f : m[i];
+            float cv = ex2(fminf(mref - mv[i] + KV8_HEAD, KV8_FLOOR + KV8_HEAD));   // (no token yet: mv is -inf)
+            const float unit = kv8_unit(fmaxf(vsc[0], vsc[1]), cv, mref);
+            float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const float c = vsc[u] * cv;
+                const float c = kv8_factor(vsc[u], cv);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     s[u][k] = ex2(s[u][k] - mref);
-                    l[i] += s[u][k];
+                    sum += s[u][k];
                     s[u][k] *= c;
                 }
                 uint32_t l0, l1;
@@ -344,6 +348,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
                     wf[u][NR - 1][i] = l0, wf[u][NR - 1][2 + i] = l1;
                 }
             }
+            l[i] = fmaf(sum, unit, l[i]);
         }
         // weights times V: byte j of the lane's piece of tokens 2t, 2t+1, 2t+8, 2t+9 is column tile j
 #pragma unroll
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     for (int i = 0; i < NR; i++) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const float back = mv[i] == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv[i] - m[i] - KV8_HEAD, 126.0f), -126.0f));
+        const float back = mv[i] == -INFINITY ? 0.0f : ex2(mv[i] - m[i] - KV8_HEAD);
         const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];   // no token: 0; NaN stays
         float *dst = so + (w * NQ + g + 8 * i) * (HD + 4);
 #pragma unroll

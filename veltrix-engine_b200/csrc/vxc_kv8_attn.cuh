@@ -29,6 +29,25 @@ struct Kv8AttnArgs {
 
 #define KV8_HEAD 10.0f   // weights up to 2^(10 + 5): in fp16's range with 2^-34 of the largest as last place
 #define KV8_LAG 5.0f
+// The weights' reference is kept within 2^KV8_FLOOR of the largest softmax weight: 2^(m - mv + KV8_HEAD)
+// and its inverse are then normal floats whatever V's scales are.  Where the floor holds, all that V adds is
+// below 2^-115 of the softmax, and weights of a scale of 2^-126 still stand at 2^-1 (24 bits above the last place).
+#define KV8_FLOOR 115.0f
+
+// Weights are w = 2^(s - ref) c, c = v_scale * cv, cv = 2^(m - mv + KV8_HEAD), and the softmax's sum adds
+// 2^(s - ref) * kv8_unit(..); ref is m on entry.  A visible token's w is at most 2^(KV8_HEAD + KV8_LAG), so
+// with a c over 2^126 (vmax: the largest v_scale in sight) the weight that goes with it has 2^(s - m) below
+// 2^-111, and with one over 2^128 may still be above 2^-126: exponentials are then taken 2^16 times
+// as large, c and the unit 2^-16 times.
+__device__ __forceinline__ float kv8_unit(float vmax, float &cv, float &ref) {
+    if (vmax * cv <= 0x1p126f) return 1.0f;
+    ref -= 16.0f;
+    cv *= 0x1p-16f;
+    return 0x1p-16f;
+}
+// What is over 2^127 even so belongs to weights below 2^-128 or to masked tokens: c stays finite, so that 0
+// times it is 0.
+__device__ __forceinline__ float kv8_factor(float v_scale, float cv) { return fminf(v_scale * cv, 0x1p127f); }
 
 template <int N>
 __device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void *src, bool have) {

@@ -462,18 +462,24 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
                 l *= ex2(m - mx);   // 0 at first
                 m = mx;
             }
-            if (mxv > mv + KV8_LAG || (mv == -INFINITY && mxv > mv)) {
+            const float least = m - KV8_FLOOR;
+            mxv = fmaxf(mxv, least);
+            if (mxv > mv + KV8_LAG || least > mv) {
                 shrink = ex2(mv - mxv);
                 mv = mxv;
             }
-            const float mref = m == -INFINITY ? 0.0f : m;
-            const float cv = ex2(fminf(mref - mv + KV8_HEAD, 120.0f));
+            float mref = m == -INFINITY ? 0.0f : m;
+            float cv = ex2(fminf(mref - mv + KV8_HEAD, KV8_FLOOR + KV8_HEAD));   // (no token yet: mv is -inf)
+            float vmax = page_vs[e][g0];
+#pragma unroll
+            for (int c = 1; c < NG; c++) vmax = fmaxf(vmax, page_vs[e][g0 + c]);
+            const float unit = kv8_unit(vmax, cv, mref);
             const uint64_t nm = f2(-mref, -mref), minus = f2(-1.0f, -1.0f);
             uint64_t sum = f2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < NG; c++) {
                 // (read again: registers are what is short here)
-                const float fg = mn_factor(f * page_ks[e][g0 + c]), cw = page_vs[e][g0 + c] * cv;
+                const float fg = mn_factor(f * page_ks[e][g0 + c]), cw = kv8_factor(page_vs[e][g0 + c], cv);
                 const uint64_t fkc = f2(fg, fg), cw2 = f2(cw, cw);
                 uint32_t w[16];
 #pragma unroll
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
             {
                 float x, y;
                 unf2(sum, x, y);
-                l += x + y;
+                l = fmaf(x + y, unit, l);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(MN_THREADS, 1) k_kv8_attn_many(const Kv8AttnAr
 #pragma unroll
             for (int i = 0; i < NP; i++) L += red[0][0][qrow + TQ * i].x + red[0][1][qrow + TQ * i].x;
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
-            const float back = mv == -INFINITY ? 0.0f : ex2(fmaxf(fminf(mv - m - KV8_HEAD, 126.0f), -126.0f));
+            const float back = mv == -INFINITY ? 0.0f : ex2(mv - m - KV8_HEAD);
             // (every product has ended: V's space is free)
 #pragma unroll
             for (int d = 0; d < HC; d += 4)
