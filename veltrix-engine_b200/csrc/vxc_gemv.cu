@@ -268,8 +268,7 @@ __global__ void __launch_bounds__(128) k_qgemv_simt(const uint8_t *__restrict__ 
 }
 
 // Activation image of x[M][K] (one CTA per row): xs[m] and the hi/lo chunks.
-__global__ void k_act_image(const float *__restrict__ x, int K, int N, uint8_t *__restrict__ img,
-                            float *__restrict__ xs) {
+__global__ void k_act_image(const float *x, int K, int N, uint8_t *img, float *xs) {
     __shared__ float red[32];
     pdl_trigger();
     pdl_wait();
@@ -311,7 +310,7 @@ int vxc_launch_act_image(const float *x, int M, int K, uint8_t *img, float *xs, 
 }
 
 // Deterministic split-K reduction: y[m][r] = sum_{s<ks} ws[s][m][r] in order.
-__global__ void k_splitk_reduce(const float *__restrict__ ws, int ks, int MR, float *__restrict__ y) {
+__global__ void k_splitk_reduce(const float *ws, int ks, int MR, float *y) {
     pdl_trigger();
     pdl_wait();
     int i = blockIdx.x * blockDim.x + threadIdx.x;

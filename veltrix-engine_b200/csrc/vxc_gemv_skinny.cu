@@ -131,8 +131,8 @@ struct SkSlot {
 
 template <int QT, int MAXM>
 __global__ void __launch_bounds__(SK_WARPS * 32, SkOcc<MAXM>::CTAS)
-    k_qgemv_skinny(const uint8_t *__restrict__ qs, int R, int nblk, float wscale, const float *__restrict__ x,
-                   int ldx, int M, float *__restrict__ out, int bps, int ks) {
+    k_qgemv_skinny(const uint8_t *__restrict__ qs, int R, int nblk, float wscale, const float *x,
+                   int ldx, int M, float *out, int bps, int ks) {
     using Sl = SkSlot<QT, MAXM>;
     constexpr int RPL = SK_RPL, ROWS = SK_UROWS;
     constexpr int QB = Sl::QB, SLOT = Sl::BYTES, S = Sl::STAGES;
@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(SK_WARPS * 32, SkOcc<MAXM>::CTAS)
 #pragma unroll
                 for (int m = 0; m < MAXM; m++)
                     if (m < M) {
-                        xr[m][0] = __ldg(reinterpret_cast<const float4 *>(xb + (size_t)m * ldx));
-                        xr[m][1] = __ldg(reinterpret_cast<const float4 *>(xb + (size_t)m * ldx) + 1);
+                        xr[m][0] = *reinterpret_cast<const float4 *>(xb + (size_t)m * ldx);
+                        xr[m][1] = *(reinterpret_cast<const float4 *>(xb + (size_t)m * ldx) + 1);
                     }
 #pragma unroll
                 for (int i = 0; i < RPL; i++) {

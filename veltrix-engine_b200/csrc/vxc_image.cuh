@@ -34,7 +34,7 @@ __device__ __forceinline__ void vxc_hilo8(const float *v, float s, uint4 &hi, ui
 // Row m of the image for a K-long row whose element k is val(k); called by
 // every thread of the CTA (any block size).
 template <class F>
-__device__ __forceinline__ void vxc_image_row(uint8_t *__restrict__ img, int N, int m, int K, float s, F val) {
+__device__ __forceinline__ void vxc_image_row(uint8_t *img, int N, int m, int K, float s, F val) {
     for (int ch = threadIdx.x; ch < K / 8; ch += blockDim.x) {
         const int b = ch >> 2, c = ch & 3;
         float v[8];

@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(256) k_gemv_kq(const uint8_t *__restrict__ w, 
 // out[m * ldo + r] for m < M, one slice (no split-K).
 template <int T>
 __global__ void __launch_bounds__(256) k_gemv_kq_img(const uint8_t *__restrict__ w, int R, int nb,
-                                                     const uint8_t *__restrict__ img, int N,
-                                                     const float *__restrict__ xs, int M, float *__restrict__ out,
+                                                     const uint8_t *img, int N,
+                                                     const float *xs, int M, float *out,
                                                      int ldo) {
     pdl_trigger();
     pdl_wait();

@@ -104,8 +104,6 @@ __device__ __forceinline__ int tb_find(const int *a, int n, int i) {
     return lo;
 }
 
-// (No __restrict__ here or below: a load through a const restricted pointer is
-// taken for one of constant data, and may be moved above griddepcontrol.wait.)
 __global__ void __launch_bounds__(TB_THREADS)
     k_kv8_tables(const int *d_len, const int *d_new, int n, int bs, int nb, int max_blocks,
                  int *table, int *d_held, int *ring, int *state,

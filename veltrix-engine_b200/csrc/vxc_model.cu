@@ -115,8 +115,10 @@ struct vxc_seqs {
 // ---------------------------------------------------------------------------
 // kernels
 // ---------------------------------------------------------------------------
+// Only pointers to what no kernel writes (weights, the RoPE table) are
+// restricted (see pdl_wait).
 __global__ void k_embed(const uint8_t *__restrict__ embd, int type, size_t row_bytes, int vocab, int E,
-                        const int *__restrict__ tokens, float *__restrict__ x, unsigned int *err) {
+                        const int *tokens, float *x, unsigned int *err) {
     pdl_trigger();
     pdl_wait();
     const int m = blockIdx.x;
@@ -200,9 +202,9 @@ __device__ __forceinline__ float block_max(float v, float *red) {
 // blockIdx.x < H: q head -> qbuf; < H + KH: k head -> cache; else v head ->
 // cache (head-major [slot][kv head][pos][hd]), or to row m of kc and vc when
 // to_rows (the paged cache's append reads them).  Thread = one (even, odd) pair.
-__global__ void k_rope_kv(Part qkv, int T, const int *__restrict__ d_slot, const int *__restrict__ d_pos,
+__global__ void k_rope_kv(Part qkv, int T, const int *d_slot, const int *d_pos,
                           const float2 *__restrict__ rope, int max_pos, int H, int KH, int hd,
-                          float *__restrict__ qbuf, float *__restrict__ kc, float *__restrict__ vc, int n_slots,
+                          float *qbuf, float *kc, float *vc, int n_slots,
                           int max_ctx, int to_rows, unsigned int *err) {
     pdl_trigger();
     pdl_wait();
@@ -277,9 +279,9 @@ __device__ __forceinline__ int attn_chunk(int r, int c) { return (c >> 3) * (ATT
 // that its 16 accumulators per lane stay in registers
 template <int HD, int QC>
 __global__ void __launch_bounds__(128, QC > 8 ? 3 : 4)
-    k_attn(const float *__restrict__ qbuf, int T, const int *__restrict__ d_slot, const int *__restrict__ d_pos,
+    k_attn(const float *qbuf, int T, const int *d_slot, const int *d_pos,
            int H, int KH, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, int row0,
-           int n_slots, int max_ctx, int SL, int nqc, float *__restrict__ part, unsigned int *err) {
+           int n_slots, int max_ctx, int SL, int nqc, float *part, unsigned int *err) {
     constexpr int NC = HD / 4;                // float4 chunks per row
     constexpr int QW = NC / 4;                // chunks per warp
     constexpr int RPW = 32 / QW;              // V rows per warp instruction in P.V
@@ -559,11 +561,11 @@ __device__ __forceinline__ void image_cols(uint8_t *img, size_t chunk_bytes, int
 //   h = w * (x[src] * (1/sqrt(sum(x^2)/E + 1e-5)))        (src/tensor.c:132-140)
 // Output row m (blockIdx.y) reads source row rows[m] (all rows when rows ==
 // NULL); x is written back only when write_x.
-__global__ void __launch_bounds__(ROW_THREADS) k_norm_image(float *__restrict__ x, Part add,
+__global__ void __launch_bounds__(ROW_THREADS) k_norm_image(float *x, Part add,
                                                               const float *__restrict__ w, int E,
-                                                              const int *__restrict__ rows, int write_x, int M_out,
-                                                              uint8_t *__restrict__ img, size_t chunk_bytes, int csh,
-                                                              float *__restrict__ xs, float *__restrict__ xf) {
+                                                              const int *rows, int write_x, int M_out,
+                                                              uint8_t *img, size_t chunk_bytes, int csh,
+                                                              float *xs, float *xf) {
     extern __shared__ float v[];   // local columns
     __shared__ float red[32], slots[2];
     cg::cluster_group cl = cg::this_cluster();
@@ -604,9 +606,9 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_image(float *__restrict__ 
 
 // f = |silu(g)| < 0.01 ? 0 : silu(g) * u  (src/model.c:580-585, src/tensor.c:71-88, :277)
 // from the fused gate/up GEMV's partials, then the image for the down GEMV.
-__global__ void __launch_bounds__(ROW_THREADS) k_swiglu_image(Part gu, int F, int M, uint8_t *__restrict__ img,
-                                                                size_t chunk_bytes, int csh, float *__restrict__ xs,
-                                                                float *__restrict__ xf) {
+__global__ void __launch_bounds__(ROW_THREADS) k_swiglu_image(Part gu, int F, int M, uint8_t *img,
+                                                                size_t chunk_bytes, int csh, float *xs,
+                                                                float *xf) {
     extern __shared__ float v[];
     __shared__ float red[32], slots[1];
     cg::cluster_group cl = cg::this_cluster();
@@ -638,10 +640,10 @@ __global__ void __launch_bounds__(ROW_THREADS) k_swiglu_image(Part gu, int F, in
 // then the image of the row for the attention-output GEMV:
 //   out = (sum_s e^{m_s-M} o_s) / (sum_s e^{m_s-M} l_s + 1e-10)   (vx_softmax's +1e-10, src/tensor.c:168)
 // One warp per head; lane s holds split s's weight e^{m_s-M}.
-__global__ void __launch_bounds__(ROW_THREADS) k_combine_image(const float *__restrict__ part, int T, int H, int KH,
-                                                                 int hd, int nsplit, int M, uint8_t *__restrict__ img,
-                                                                 size_t chunk_bytes, int csh, float *__restrict__ xs,
-                                                                 float *__restrict__ xf) {
+__global__ void __launch_bounds__(ROW_THREADS) k_combine_image(const float *part, int T, int H, int KH,
+                                                                 int hd, int nsplit, int M, uint8_t *img,
+                                                                 size_t chunk_bytes, int csh, float *xs,
+                                                                 float *xf) {
     extern __shared__ float v[];
     __shared__ float red[32], slots[1];
     cg::cluster_group cl = cg::this_cluster();
@@ -696,9 +698,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_combine_image(const float *__re
     cl.sync();
 }
 
-// The paged cache's row kernels.  (No __restrict__: a load through a const
-// restricted pointer may be moved above griddepcontrol.wait, and k_kv8_rows then
-// read the state of the tables before they were made.)
+// The paged cache's row kernels.
 // Row m of x[M][W] (W = H hd) as the operand of the attention-output GEMV: the
 // paged cache's attention writes finished rows.
 __global__ void __launch_bounds__(ROW_THREADS) k_rows_image(const float *x, int W, int M,
@@ -783,7 +783,7 @@ __global__ void k_kv8_rows(const int *seq, const int *d_pos, int M, int T, int m
 }
 
 // logits[m][w*Vl + v] = gathered[w][m][v]: the vocabulary shards of the GPUs side by side
-__global__ void k_vocab_gather(const float *__restrict__ all, int world, int n_rows, int Vl, float *__restrict__ out) {
+__global__ void k_vocab_gather(const float *all, int world, int n_rows, int Vl, float *out) {
     pdl_trigger();
     pdl_wait();
     const size_t V = (size_t)world * Vl, tot = (size_t)n_rows * V;
@@ -796,7 +796,7 @@ __global__ void k_vocab_gather(const float *__restrict__ all, int world, int n_r
 // Greedy token of one logits row, the reference's rule (src/main.c:307-311):
 // scanning upward from max = -1e30, the first index whose value is strictly
 // greater than every earlier one (NaN never wins; 0 when none exceeds -1e30).
-__global__ void __launch_bounds__(1024) k_argmax_row(const float *__restrict__ lg, int V, int *__restrict__ tok) {
+__global__ void __launch_bounds__(1024) k_argmax_row(const float *lg, int V, int *tok) {
     pdl_trigger();
     pdl_wait();
     float best = -1e30f;
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(1024) k_argmax_row(const float *__restrict__ l
 // One step of the greedy loop after the argmax: the token just forwarded is
 // now cached (pos + 1); the new token ends the loop if it is eos, else it is
 // emitted.  st = {emitted, next position, done}.
-__global__ void k_greedy_record(const int *__restrict__ tok, int *__restrict__ st, int *__restrict__ out, int eos,
+__global__ void k_greedy_record(const int *tok, int *st, int *out, int eos,
                                 int max_tokens) {
     pdl_trigger();
     pdl_wait();
@@ -847,7 +847,7 @@ __global__ void k_greedy_record(const int *__restrict__ tok, int *__restrict__ s
 }
 
 // logits[m][r] = sum of the LM head's partials
-__global__ void k_part_out(Part p, int n_rows, float *__restrict__ out) {
+__global__ void k_part_out(Part p, int n_rows, float *out) {
     pdl_trigger();
     pdl_wait();
     const size_t n = (size_t)n_rows * p.R;

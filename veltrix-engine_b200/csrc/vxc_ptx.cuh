@@ -116,6 +116,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, int 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- programmatic dependent launch ---------------------------------------
+// In a kernel that waits, a parameter is __restrict__ only if no kernel writes
+// what it points to, and other data are not read by __ldg: such loads count as
+// loads of constant data, and the compiler may move them above the wait (a
+// kernel of the paged cache read its predecessor's input that way).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
