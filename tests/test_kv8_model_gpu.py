@@ -152,3 +152,59 @@ def test_contexts_over_the_limit_are_refused(cuda):
         h = ctypes.c_void_p()
         assert s.L.vxc_seqs_create_kv8(s.net, 1, max_ctx, 64, INT8, 64, 4, ctypes.byref(h)) == -4 and not h.value
     s.close()
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+def test_greedy_ended_by_eos_leaves_the_cache_as_the_host_loop_does(cuda, kind):
+    """The replays between eos and the host's next look at the device change nothing: logits after an ended
+    generation are those after the same tokens one by one."""
+    import vxb200
+    m = vxb200.Model(fixtures.path("tiny_target"))
+    vocab = fixtures.CONFIGS["tiny_target"][5]
+    for seed in range(6):
+        ids = np.random.default_rng(seed).integers(0, vocab, 8).astype(np.int32)
+        prompt, more = ids[:2 + seed], ids[-2:]
+        m.set_kv_cache(kind)
+        stream = m.generate_greedy(prompt, 24)
+        for end in (1, 3, 6):
+            eos = int(stream[end])
+            n = int(np.argmax(stream == eos))
+            m.set_kv_cache(kind)
+            np.testing.assert_array_equal(m.generate_greedy(prompt, 24, eos), stream[:n])
+            assert m.cache_len == len(prompt) + n
+            got = m.forward(more)
+            m.set_kv_cache(kind)
+            m.forward(prompt)
+            for t in stream[:n]:
+                m.forward(np.array([t], np.int32))
+            np.testing.assert_array_equal(got, m.forward(more))
+    m.close()
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+def test_greedy_ended_by_eos_needs_no_more_blocks(cuda, kind):
+    """eos with the last position at a block's end and no block free."""
+
+    def run(s, prompt, eos, most=20):
+        out, n, pos = np.zeros(most, np.int32), ctypes.c_int(-1), ctypes.c_int(-1)
+        rc = s.L.vxc_greedy_generate(s.s, 0, 0, prompt.ctypes.data, len(prompt), out.ctypes.data, most, eos,
+                                     ctypes.byref(n), ctypes.byref(pos))
+        return rc, out[:max(n.value, 0)], pos.value
+
+    cases = 0
+    for n in range(1, 7):   # tokens before eos
+        prompt = np.random.default_rng(n).integers(0, 4096, 32 - n).astype(np.int32)
+        s = Seqs(cuda, kind, 1, 256, 64)
+        rc, stream, _ = run(s, prompt, -1)
+        s.close()
+        assert rc == 0
+        if stream[n] in stream[:n]:
+            continue
+        cases += 1
+        s = Seqs(cuda, kind, 1, 256, 64, n_blocks=2)
+        rc, got, pos = run(s, prompt, int(stream[n]))
+        assert rc == 0, s.L.vxc_error_string()
+        np.testing.assert_array_equal(got, stream[:n])
+        assert pos == 32
+        s.close()
+    assert cases

@@ -202,10 +202,12 @@ __device__ __forceinline__ float block_max(float v, float *red) {
 // blockIdx.x < H: q head -> qbuf; < H + KH: k head -> cache; else v head ->
 // cache (head-major [slot][kv head][pos][hd]), or to row m of kc and vc when
 // to_rows (the paged cache's append reads them).  Thread = one (even, odd) pair.
+// Rows of a slot or position outside the set are left out; that is an error
+// unless idle_ok says that a negative slot is a group with nothing to do.
 __global__ void k_rope_kv(Part qkv, int T, const int *d_slot, const int *d_pos,
                           const float2 *__restrict__ rope, int max_pos, int H, int KH, int hd,
                           float *qbuf, float *kc, float *vc, int n_slots,
-                          int max_ctx, int to_rows, unsigned int *err) {
+                          int max_ctx, int to_rows, int idle_ok, unsigned int *err) {
     pdl_trigger();
     pdl_wait();
     const int head = blockIdx.x, m = blockIdx.y, p = threadIdx.x;
@@ -214,7 +216,7 @@ __global__ void k_rope_kv(Part qkv, int T, const int *d_slot, const int *d_pos,
     const int pos = d_pos[g] + t;
     const int E = H * hd, kvd = KH * hd;
     if (pos < 0 || pos >= max_ctx || pos >= max_pos || slot < 0 || slot >= n_slots) {
-        if (head == 0 && p == 0) vxc_flag_error(err, VXC_DERR_CTX_FULL);
+        if (head == 0 && p == 0 && !(idle_ok && slot < 0)) vxc_flag_error(err, VXC_DERR_CTX_FULL);
         return;
     }
     if (2 * p >= hd) return;
@@ -829,21 +831,23 @@ __global__ void __launch_bounds__(1024) k_argmax_row(const float *lg, int V, int
 
 // One step of the greedy loop after the argmax: the token just forwarded is
 // now cached (pos + 1); the new token ends the loop if it is eos, else it is
-// emitted.  st = {emitted, next position, done}.
+// emitted.  st = {emitted, next position, done}.  *slot (unless NULL), the slot
+// of the loop's forward, becomes -1 when the loop has ended.
 __global__ void k_greedy_record(const int *tok, int *st, int *out, int eos,
-                                int max_tokens) {
+                                int max_tokens, int *slot) {
     pdl_trigger();
     pdl_wait();
     if (threadIdx.x != 0 || st[2]) return;
     st[1] += 1;
     const int t = *tok;
-    if (t == eos) {
-        st[2] = 1;
-        return;
+    if (t != eos) {
+        out[st[0]] = t;
+        st[0] += 1;
     }
-    out[st[0]] = t;
-    st[0] += 1;
-    if (st[0] >= max_tokens) st[2] = 1;
+    if (t == eos || st[0] >= max_tokens) {
+        st[2] = 1;
+        if (slot) *slot = -1;
+    }
 }
 
 // logits[m][r] = sum of the LM head's partials
@@ -1754,9 +1758,10 @@ static int gemv_rows(vxc_seqs *s, const vxc_qmat *w, int M, Part *out, cudaStrea
 }
 
 // The forward of vxc_forward; matrices multiply M >= gemm_min rows on the GEMM.
+// idle_ok (paged cache): groups of a negative slot are left out without an error.
 static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, const int *d_pos, int n_groups,
                         int rows_per_group, const int *d_logit_rows, int n_logit_rows, float *d_logits,
-                        void *stream, int gemm_min) {
+                        void *stream, int gemm_min, int idle_ok = 0) {
     if (!s || !d_tokens || !d_slot || !d_pos || n_groups <= 0 || rows_per_group <= 0) {
         vxc_set_error("vxc_forward: bad arguments");
         return -4;
@@ -1872,7 +1877,7 @@ static int forward_impl(vxc_seqs *s, const int *d_tokens, const int *d_slot, con
         prof_end(2, pe, st);
         pe = prof_begin(st);
         e = launch_pdl(k_rope_kv, dim3(H + 2 * KH, M), dim3(((hd / 2) + 31) / 32 * 32), 0, st, pp, T, d_slot, d_pos, (const float2 *)n->rope,
-                       c.max_pos, H, KH, hd, s->qbuf, kc, vc, s->n_slots, s->max_ctx, paged ? 1 : 0, err);
+                       c.max_pos, H, KH, hd, s->qbuf, kc, vc, s->n_slots, s->max_ctx, paged ? 1 : 0, idle_ok, err);
         vxc_kv8 kv = s->kv8;
         if (paged) {   // this layer's blocks
             const size_t skip = (size_t)l * kv.n_blocks * KH;
@@ -2064,6 +2069,11 @@ extern "C" int vxc_greedy_generate(vxc_seqs *s, int slot, int pos0, const int *h
         rc = vxc_forward(s, d_i, d_i + o_meta, d_i + o_meta + 1, 1, n, last ? d_i + o_meta + 2 : NULL, last ? 1 : 0,
                          last ? d_l : NULL, st);
     }
+    // the loop's forwards after eos: in the fp32 cache they write only the position past the last one;
+    // in a paged cache they would change the block of the positions before it (and may need another
+    // block), so there they get no slot
+    const int paged = s->kv8.type != 0;
+    int *end_slot = paged ? d_i + o_slot : NULL;
     int state[3] = {0, pos0 + n_prompt - 1, 0};
     if (rc == 0) {
         const int init[6] = {state[0], state[1], state[2], slot, 0, 0};
@@ -2071,7 +2081,7 @@ extern "C" int vxc_greedy_generate(vxc_seqs *s, int slot, int pos0, const int *h
         if (e == cudaSuccess) e = launch_pdl(k_argmax_row, dim3(1), dim3(1024), 0, st, (const float *)d_l, V, d_i + o_tok);
         if (e == cudaSuccess)
             e = launch_pdl(k_greedy_record, dim3(1), dim3(32), 0, st, (const int *)(d_i + o_tok), d_i + o_st,
-                           d_i + o_out, eos_id, max_tokens);
+                           d_i + o_out, eos_id, max_tokens, end_slot);
         if (e == cudaSuccess) e = cudaMemcpyAsync(state, d_i + o_st, sizeof state, cudaMemcpyDeviceToHost, st);
         if (e == cudaSuccess) e = cudaStreamSynchronize(st);
         if (e != cudaSuccess) { vxc_set_error("vxc_greedy_generate: %s", cudaGetErrorString(e)); rc = -3; }
@@ -2081,12 +2091,13 @@ extern "C" int vxc_greedy_generate(vxc_seqs *s, int slot, int pos0, const int *h
         const long long before = vxc_launch_count();
         e = cudaStreamBeginCapture(st, cudaStreamCaptureModeRelaxed);
         if (e == cudaSuccess) {
-            rc = vxc_forward(s, d_i + o_tok, d_i + o_slot, d_i + o_st + 1, 1, 1, d_i + o_row, 1, d_l, st);
+            rc = forward_impl(s, d_i + o_tok, d_i + o_slot, d_i + o_st + 1, 1, 1, d_i + o_row, 1, d_l, st,
+                              VXC_GEMM_MIN_ROWS, paged);
             cudaError_t e1 = cudaSuccess, e2 = cudaSuccess;
             if (rc == 0) e1 = launch_pdl(k_argmax_row, dim3(1), dim3(1024), 0, st, (const float *)d_l, V, d_i + o_tok);
             if (rc == 0 && e1 == cudaSuccess)
                 e1 = launch_pdl(k_greedy_record, dim3(1), dim3(32), 0, st, (const int *)(d_i + o_tok), d_i + o_st,
-                                d_i + o_out, eos_id, max_tokens);
+                                d_i + o_out, eos_id, max_tokens, end_slot);
             e2 = cudaStreamEndCapture(st, &graph);
             e = e1 != cudaSuccess ? e1 : e2;
         }
@@ -2095,8 +2106,7 @@ extern "C" int vxc_greedy_generate(vxc_seqs *s, int slot, int pos0, const int *h
         if (rc == 0 && e == cudaSuccess) e = cudaGraphInstantiate(&exec, graph, 0);
         if (rc == 0 && e != cudaSuccess) { vxc_set_error("vxc_greedy_generate: graph: %s", cudaGetErrorString(e)); rc = -3; }
         // each replay emits one token until done: max_tokens - 1 replays at most; the
-        // host looks at the done flag every 8 replays (a few extra forwards after
-        // eos write only positions past the cache length)
+        // host looks at the done flag every 8 replays
         for (int i = 0; rc == 0 && i < max_tokens - 1; i++) {
             e = cudaGraphLaunch(exec, st);
             if (e != cudaSuccess) break;
