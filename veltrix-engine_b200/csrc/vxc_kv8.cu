@@ -3,8 +3,8 @@
 // (No reference counterpart: the reference keeps one contiguous fp32 cache,
 // src/model.c:404-411.)
 #include "vxc_kv8.cuh"
+#include "vxc_smem_limit.h"
 
-#include <atomic>
 #include <climits>
 #include <cooperative_groups.h>
 
@@ -40,38 +40,24 @@ int vxc_kv8_check(const vxc_kv8 *kv, const char *who) {
     return 0;
 }
 
-// The limit is per kernel and device and only ever raised; a kernel that has
-// it on a device is remembered, since asking costs a launch's time.
-cudaError_t kv8_allow_smem(const void *kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return cudaSuccess;
-    struct Entry {
-        std::atomic<const void *> kernel;
-        std::atomic<size_t> bytes[64];
-    };
-    static Entry seen[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    Entry *own = nullptr;
-    for (Entry &s : seen) {
-        const void *k = s.kernel.load(std::memory_order_acquire);
-        if (!k && s.kernel.compare_exchange_strong(k, kernel)) k = kernel;
-        if (k == kernel) {
-            own = &s;
-            break;
-        }
+namespace {
+struct Runtime {   // for vxc_smem_allow
+    typedef cudaError_t error;
+    static constexpr cudaError_t ok = cudaSuccess;
+    static cudaError_t device(int *d) { return cudaGetDevice(d); }
+    static cudaError_t limit(const void *kernel, size_t *bytes) {
+        cudaFuncAttributes fa;
+        const cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+        if (e == cudaSuccess) *bytes = (size_t)fa.maxDynamicSharedSizeBytes;
+        return e;
     }
-    if (own && dev < 64 && own->bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kernel);
-    if (e == cudaSuccess && (size_t)fa.maxDynamicSharedSizeBytes < bytes)
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess && own && dev < 64) {
-        size_t have = own->bytes[dev].load();
-        while (have < bytes && !own->bytes[dev].compare_exchange_weak(have, bytes)) {}
+    static cudaError_t set_limit(const void *kernel, size_t bytes) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     }
-    return e;
-}
+};
+}  // namespace
+
+cudaError_t kv8_allow_smem(const void *kernel, size_t bytes) { return vxc_smem_allow<Runtime>(kernel, bytes); }
 
 // ---------------------------------------------------------------------------
 // block tables and slot maps
