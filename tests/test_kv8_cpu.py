@@ -75,6 +75,17 @@ def test_tables_refusals(bad):
     assert tables(**bad) == PARAM
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_integer_arrays_are_refused(off):
+    for name in ("length", "new", "table", "held", "ring", "state", "row0", "slot"):
+        assert tables(**{name: BUF + off}) == PARAM, name
+        assert b"vxc_kv8_tables" in vxb200.lib().vxc_error_string()
+    assert append(cache(), slot=BUF + off) == PARAM
+    for name in ("table", "row0", "pos"):
+        assert attn(cache(), **{name: BUF + off}) == PARAM, name
+        assert b"vxc_kv8_attn" in vxb200.lib().vxc_error_string()
+
+
 def test_without_a_device_every_call_is_unsupported():
     if vxb200.lib().vxc_device_count() > 0:
         pytest.skip("a CUDA device is present")

@@ -258,8 +258,9 @@ __global__ void __launch_bounds__(TB_THREADS)
 extern "C" int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks,
                               int max_blocks, int *d_table, int *d_held, int *d_free, int *d_state, int n_rows,
                               int *d_row0, int *d_slot, void *stream) {
-    if (!d_len || !d_new || !d_table || !d_held || !d_free || !d_state || !d_row0 || (n_rows > 0 && !d_slot)) {
-        vxc_set_error("vxc_kv8_tables: an array is missing");
+    if (!d_len || !d_new || !d_table || !d_held || !d_free || !d_state || !d_row0 || (n_rows > 0 && !d_slot) ||
+        !kv8_words(d_len, d_new, d_table, d_held, d_free, d_state, d_row0, d_slot)) {
+        vxc_set_error("vxc_kv8_tables: an array is missing or not aligned");
         return -4;
     }
     if (n_req < 1 || n_req > VXC_KV8_MAX_REQ || n_rows < 0 || n_rows > KV8_MAX_TOKENS) {
@@ -522,8 +523,8 @@ extern "C" int vxc_kv8_append(const vxc_kv8 *kv, const float *k, long long ldk, 
     }
     const long long width = (long long)kv->n_kv_heads * kv->head_dim;
     if (n_rows > 0 && (!k || !v || !d_slot || (uintptr_t)k % 16 || (uintptr_t)v % 16 || ldk < width || ldv < width ||
-                       ldk % 4 || ldv % 4)) {
-        vxc_set_error("vxc_kv8_append: rows missing, not 16-byte aligned, or shorter than %lld floats", width);
+                       ldk % 4 || ldv % 4 || !kv8_words(d_slot))) {
+        vxc_set_error("vxc_kv8_append: rows or slots missing or not aligned, or rows shorter than %lld floats", width);
         return -4;
     }
     if (int rc = vxc_require_device()) return rc;

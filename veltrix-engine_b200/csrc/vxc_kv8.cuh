@@ -84,5 +84,8 @@ static cudaError_t kv8_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t
 
 // Lets `kernel` be launched with `bytes` of dynamic shared memory on the current device.
 cudaError_t kv8_allow_smem(const void *kernel, size_t bytes);
+// Whether an address can be that of ints or floats (a misaligned one would fault on the device).
+template <typename... P>
+static inline bool kv8_words(const P *...p) { return ((((uintptr_t)p % 4) == 0) && ...); }
 // 0, or -4 with the error set: the fields of a cache (host side).
 int vxc_kv8_check(const vxc_kv8 *kv, const char *who);

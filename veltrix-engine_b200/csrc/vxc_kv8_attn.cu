@@ -713,7 +713,7 @@ extern "C" int vxc_kv8_attn(const vxc_kv8 *kv, const float *q, long long ldq, in
                             size_t workspace_bytes, void *stream) {
     if (int rc = attn_check(kv, n_heads, n_req, n_rows, max_new, max_blocks)) return rc;
     const long long width = (long long)n_heads * kv->head_dim;
-    if (!d_table || !d_row0 || !d_pos ||
+    if (!d_table || !d_row0 || !d_pos || !kv8_words(d_table, d_row0, d_pos) ||
         (n_rows > 0 && (!q || !out || (uintptr_t)q % 16 || (uintptr_t)out % 16 || ldq < width || ldo < width ||
                         ldq % 4 || ldo % 4))) {
         vxc_set_error("vxc_kv8_attn: an array is missing or not aligned, or rows are shorter than %lld floats", width);
