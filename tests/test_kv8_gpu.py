@@ -614,3 +614,31 @@ def test_two_calls_at_once_on_two_streams(cuda):
     torch.cuda.synchronize()
     for w, a in zip(want, args):
         np.testing.assert_array_equal(a[4].cpu().numpy().reshape(w.shape), w)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_two_calls_at_once_with_records_of_splits(cuda, new):
+    """As above with contexts whose splits meet in the workspaces: over 8 splits of a few queries, split tiles."""
+    torch = cuda
+    rng = np.random.default_rng(new)
+    runs = []
+    for s in range(2):
+        lens = np.array([25600 - new], np.int32)
+        table, nb = paged(rng, lens + new, 64)
+        d = Dev(torch, E4M3, nb, 64, 1, 64, seed=s)
+        q = rng.standard_normal((new, 2, 64)).astype(np.float32)
+        row0 = np.array([0, new], np.int32)
+        want = d.attn(q, 0.1, table, row0, lens)
+        size = d.c.attn_workspace_bytes(2, 1, new, new, table.shape[1])
+        assert size > 0
+        t = [torch.from_numpy(x).cuda() for x in (q.reshape(new, -1), table, row0, lens)]
+        runs.append((d, t, torch.empty(size // 4 + 4, device="cuda"), size, torch.zeros(new, 128, device="cuda"),
+                     torch.cuda.Stream(), want, table.shape[1]))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for d, t, ws, size, out, st, want, mb in runs:
+            d.c.attn(t[0].data_ptr(), 128, 2, 0.1, t[1].data_ptr(), mb, t[2].data_ptr(), t[3].data_ptr(), 1, new, new,
+                     out.data_ptr(), 128, ws.data_ptr(), size, st.cuda_stream)
+    torch.cuda.synchronize()
+    for d, t, ws, size, out, st, want, mb in runs:
+        np.testing.assert_array_equal(out.cpu().numpy().reshape(want.shape), want)

@@ -208,3 +208,19 @@ def test_greedy_ended_by_eos_needs_no_more_blocks(cuda, kind):
         assert pos == 32
         s.close()
     assert cases
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+def test_paged_cache_of_a_tensor_parallel_model(cuda, kind):
+    """A model made by vx_model_create_tp for one GPU, its exchanges included, gives the plain model's numbers."""
+    import vxb200
+    ids = np.random.default_rng(3).integers(0, fixtures.CONFIGS["tiny_target"][5], 90).astype(np.int32)
+    got = []
+    for tp in (None, (0, 1, vxb200.tp_unique_id())):
+        m = vxb200.Model(fixtures.path("tiny_target"), tp=tp)
+        m.set_kv_cache(kind)
+        got.append([m.forward(ids[:80]), m.forward(ids[80:85]), m.generate_greedy(ids[85:], 20), m.forward(ids[:1])])
+        m.close()
+    for a, b in zip(*got):
+        assert err(b, a) <= 1e-5
+    np.testing.assert_array_equal(got[0][2], got[1][2])
