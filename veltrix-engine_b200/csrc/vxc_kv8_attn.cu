@@ -558,6 +558,10 @@ struct AttnPlan {
 #define ATTN_FEW_MAX 16   // queries of a request and kv head up to which k_kv8_attn_few is used
 #endif
 
+// The host knows the width of the table, not the lengths behind it: they are taken as spread evenly from
+// nothing to that width.
+#define ATTN_FILL 0.5
+
 static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
     AttnPlan p;
     p.chunks = 1;
@@ -584,7 +588,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
             const double places = i <= 8 ? 4 + 12.0 * (i - 1) : 6.0 * i;
             const long long room = i == 1 || i > 8 ? 296 / i : 8 * (32 / i);   // units that fit at once
             const double all = n_req == 1 ? (units + room - 1) / room * cta
-                                          : units * (places + 0.5 * 0.0144 * byte * tokens) / 296 + 0.25 * cta;
+                                          : units * (places + ATTN_FILL * 0.0144 * byte * tokens) / 296 + 0.25 * cta;
             const double time = cta > all || units <= room ? cta : all;
             if (i == 1 || time < best) best = time, S = i;
         }
@@ -599,7 +603,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         units = (some > busy ? some : busy) * kv->n_kv_heads;
         // A CTA costs about 11 us and 1.86 us per 128 tokens, one fits an SM; the join 3 us and its
         // records' way.  The S of the least time, as long as the longest CTA and as all of them on
-        // 148 SMs: requests begin longest first and have 0.6 of the tokens on average; a single one has
+        // 148 SMs: requests begin longest first and have ATTN_FILL of the tokens on average; a single one has
         // them all, and then CTAs come in whole rounds.  Measured (us, S = 1, 2, ...): 96 units of 8192
         // tokens 129, 78, 83; 64 units 128, 76, 59, 58, 62; 256 units of 4096 89, 112, 123; 200 units of
         // 16384 255, 212, 219; 128 units of 2000 39, 44, 54.
@@ -607,7 +611,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         S = 1;
         for (int i = 1; i <= 64; i++) {
             const double cta = 11 + 0.0145 * tokens / i;
-            const double all = n_req == 1 ? (units * i + 147) / 148 * cta : units * (11.0 * i + 0.6 * 0.0145 * tokens) / 148;
+            const double all = n_req == 1 ? (units * i + 147) / 148 * cta : units * (11.0 * i + ATTN_FILL * 0.0145 * tokens) / 148;
             const double join = i == 1 ? 0 : 3 + 2e-6 * n_rows * n_heads * i * (kv->head_dim + 4);
             const double time = (cta > all ? cta : all) + join;
             if (i == 1 || time < best) best = time, S = i;
@@ -619,7 +623,7 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         const long long chunks = (most + 15) / 16;
         const double byte = kv->head_dim / 128.0, cta = 4 + 0.0125 * byte * tokens;
         const int places = 148 * (kv->head_dim >= 96 ? 2 : kv->head_dim == 64 ? 3 : 4);
-        const double all = (double)n_req * kv->n_kv_heads * chunks * (6.5 + 0.75 * 0.0144 * byte * tokens) / places + 0.25 * cta;
+        const double all = (double)n_req * kv->n_kv_heads * chunks * (6.5 + ATTN_FILL * 0.0144 * byte * tokens) / places + 0.25 * cta;
         if (tokens <= 8192 && chunks * n_req <= 65535 && (cta > all ? cta : all) < 0.8 * best) {
             p.nq = 16;
             p.chunks = (int)chunks;
