@@ -27,8 +27,9 @@
  * vx_model_set_kv_cache (additive) how the model's KV cache is held from its
  *                   next forward on: 0 fp32 (as created), VXC_KV8_INT8 (1) or
  *                   VXC_KV8_E4M3 (2) the paged 8-bit cache of
- *                   include/veltrix_cuda.h.  The present cache is dropped and
- *                   cache_len set to 0.  Speculative states keep fp32 caches
+ *                   include/veltrix_cuda.h (what a call's logits depend on
+ *                   besides its tokens stands there, at vxc_seqs_create_kv8).
+ *                   The present cache is dropped and cache_len set to 0.  Speculative states keep fp32 caches
  *                   of their own.  VX_ERR_PARAM for another type.
  */
 #ifndef VX_MODEL_H

@@ -198,7 +198,10 @@ int vxc_seqs_create(const vxc_net *net, int n_slots, int max_ctx, int max_rows, 
  * nothing.  One forward takes one group per slot (a second one is left out and
  * raises the error word; n_groups <= n_slots).  n_slots <= VXC_KV8_MAX_REQ.
  * vxc_forward, vxc_forward_host and vxc_greedy_generate use either kind;
- * logits differ from the fp32 cache's by the rounding of K and V to 8 bits. */
+ * logits differ from the fp32 cache's by the rounding of K and V to 8 bits, and
+ * depend, within that rounding, on how the tokens were cut into calls and on
+ * tokens that were written and dropped before (vxc_kv8_append): decoding
+ * with drafts is not token for token decoding without. */
 int vxc_seqs_create_kv8(const vxc_net *net, int n_slots, int max_ctx, int max_rows, int kv_type, int block_size,
                         int n_blocks, vxc_seqs **out);
 void vxc_seqs_destroy(vxc_seqs *s);
@@ -282,8 +285,9 @@ int vxc_accept(const float *P, long long p_seq, long long p_pos, const float *Q,
  * All arrays are device memory of the calling thread's current device (k and v
  * 16-byte aligned, the others by their element type); nothing is copied to the
  * host and nothing is allocated, so every call can be captured in a CUDA
- * graph.  Calls are ordered by their streams only: a call that writes a cache
- * or a table may not overlap another call on the same one.
+ * graph, once vxc_device_init has made the device's error word.  Calls are
+ * ordered by their streams only: a call that writes a cache or a table may not
+ * overlap another call on the same one.
  * Out-of-range device data (a slot, a table entry, a length) never leads to an
  * access outside the arrays; it raises the device error word, as stated at
  * each call. */
@@ -316,6 +320,8 @@ typedef struct {
  * than needed; 2: a request longer than max_blocks blocks; 3: a negative
  * length, more than n_rows new tokens, or held blocks and a queue that do not
  * fit n_blocks (2 and 3 also raise the device error word).
+ * A block outside the cache that comes from the queue or a table raises the
+ * error word, and the slots of its tokens are -1; d_state[2] stays 0.
  * One launch. */
 #define VXC_KV8_MAX_REQ 8192
 int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int block_size, int n_blocks, int max_blocks,
@@ -332,8 +338,13 @@ int vxc_kv8_tables(const int *d_len, const int *d_new, int n_req, int block_size
  *   if s grew from a scale > 0, the block's other codes are rounded again to
  *       code * old / s;
  *   the rows' codes are x / s to nearest, ties to even, and the scale is s.
- * (Powers of two: dividing by s is exact, a growing scale shifts the codes, so
- * an element is off by at most one step of s however often s grew.)
+ * (Powers of two: dividing by s is exact and a growing scale shifts the codes.
+ * However often s grew, an INT8 element is off by less than s, an E4M3 element x
+ * by at most 2^-4 |x| + 2^-9 s.)
+ * A scale never shrinks before its block starts anew, and codes that were rounded
+ * again stay so: tokens that are dropped and written over (rejected drafts)
+ * leave their magnitude behind, and what a block holds depends on how its tokens
+ * were cut into calls, within these bounds.
  * The rows of one block stand together in d_slot, with no other or skipped
  * row between them, as vxc_kv8_tables writes them; of two rows with the same slot
  * the later one is kept.  A slot outside the cache is skipped and raises the
@@ -357,9 +368,10 @@ size_t vxc_kv8_attn_workspace_bytes(const vxc_kv8 *kv, int n_heads, int n_req, i
  * over the request's tokens j <= position, kv head h / (n_heads / kv heads)
  * (reference src/model.c:299-338 over its fp32 cache).  fp32 in and out,
  * q rows of ldq and out rows of ldo floats (16-byte aligned, ld a multiple of
- * 4); out may not overlap q.  Products are exact to fp32 level: codes are
- * exact in fp16, queries and weights are split into two fp16 parts, sums and
- * softmax are fp32.
+ * 4); out may not overlap q.  Codes are exact in fp16, queries and softmax
+ * weights are split into two fp16 parts (22 bits), sums and the softmax are
+ * fp32; tokens whose weight is below 2^-126 of the row's largest may count as
+ * none.  V's scales may be zero, any power of two or far apart.
  * (n_rows <= VXC_KV8_MAX_ROWS, n_rows * n_heads < 2^31, max_blocks * block_size
  * <= 2^30.)
  * A row whose position is negative sees no token and is set to 0.  Rows behind

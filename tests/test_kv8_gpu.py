@@ -513,6 +513,38 @@ def test_tables_refused_calls_change_nothing(cuda):
             assert cuda.equal(a, b), (i, bad)
 
 
+def test_tables_blocks_outside_the_cache_are_reported(cuda):
+    """From the queue, and in a table: their tokens have no slot."""
+    import vxb200
+    for i, at, bad in ((2, 6, 8), (2, 6, -3), (0, (1, 0), 99)):
+        T = Tables(cuda, 2, 16, 8, 4, front=5)   # 4 blocks to the first step: ring entries 5, 6, 7, 0
+        if i == 0:
+            assert T.step([0, 0], [20, 20], 40) == 0
+        T.dev[i][at] = bad
+        length, new = ([0, 0], [20, 20]) if i == 2 else ([20, 20], [4, 4])
+        ld, nd = (cuda.tensor(x, dtype=cuda.int32, device="cuda") for x in (length, new))
+        row0, slot = (cuda.full((n,), -9, dtype=cuda.int32, device="cuda") for n in (3, 40))
+        vxb200.kv8_tables(ld.data_ptr(), nd.data_ptr(), 2, 16, 8, 4, *(x.data_ptr() for x in T.dev), 40,
+                          row0.data_ptr(), slot.data_ptr())
+        want = kv8ref.tables(length, new, 16, 8, *T.ref, 40)
+        got = slot.cpu().numpy()
+        assert int(T.dev[3][2]) == 0 and np.array_equal(row0.cpu().numpy(), want[0])
+        if i == 2:   # the second block taken: the first request's tokens 16 to 19
+            assert error_word() == BAD_BLOCK
+            assert np.all(got[16:20] == -1)
+            keep = np.r_[0:16, 20:40]
+            np.testing.assert_array_equal(got[keep], want[1][keep])
+        else:        # the second request's first block holds none of its new tokens 20 to 23
+            np.testing.assert_array_equal(got, want[1])
+            T.dev[0][1, 1] = bad
+            vxb200.kv8_tables(ld.data_ptr(), nd.data_ptr(), 2, 16, 8, 4, *(x.data_ptr() for x in T.dev), 40,
+                              row0.data_ptr(), slot.data_ptr())
+            assert error_word() == BAD_BLOCK
+            got = slot.cpu().numpy()
+            assert np.all(got[4:8] == -1)
+            np.testing.assert_array_equal(got[:4], want[1][:4])
+
+
 # ---- together ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", [INT8, E4M3])

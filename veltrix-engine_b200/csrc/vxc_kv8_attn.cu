@@ -47,10 +47,12 @@ namespace cg = cooperative_groups;
 // The blocks and scales of the split are looked up once, at the start.
 //
 // Measured (heads of 128): 33 requests of one row behind up to 16384 tokens, 64
-// heads over 8, 100 us, 5.4 TB/s of the cache's bytes; 8 requests of 5 rows
-// behind up to 768 tokens, 32 heads, 13.6 us; 8 of one row, 32 heads of 64 over
-// 4, 7.4 us.  Bound: bytes for long contexts (issue slots 40 %, tensor pipe
-// 33 % busy); a CTA's latencies, about 4 us, for short ones.
+// heads over 8, 102 us one call after the other, 5.3 TB/s of the cache's bytes
+// (108 us among other work); 8 requests of 5 rows behind up to 768 tokens, 32
+// heads, 13.9 us; 8 of one row, 32 heads of 64 over 4, 7.6 us.  Bound: bytes for
+// long contexts (issue slots 40 %, tensor pipe 33 % busy).  Short ones: a CTA's
+// latencies, about 4 us, and its warps' chain of scores, maxima, weights and
+// products, 1.6 us per piece of 32 tokens with two warps per scheduler.
 // ---------------------------------------------------------------------------
 #define FEW_STAGES 2     // 32-token pieces per warp: one in use, one in flight (3: no faster, 4: fewer CTAs per SM, slower)
 
@@ -559,7 +561,10 @@ struct AttnPlan {
 #endif
 
 // The host knows the width of the table, not the lengths behind it: they are taken as spread evenly from
-// nothing to that width.
+// nothing to that width.  Where they are not (us; table as wide as the longest request, of 4096, of 16384
+// tokens): 8 requests of 5 rows behind 763 tokens, 32 heads, 14.7, 23, 23; 8 of one row, 32 heads of 64 over 4,
+// 7.5, 7.7, 7.7; 8 of 17 rows 36, 37, 37; 32 of 7 rows, all behind 4089 tokens, 64 heads over 8, 133 or, with
+// one block more, 145, 146; 100 of 26 rows in 26 tokens, 28 heads of 32, 62, 59, 131.
 #define ATTN_FILL 0.5
 
 static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows, int max_new, int max_blocks) {
@@ -601,7 +606,8 @@ static AttnPlan attn_plan(const vxc_kv8 *kv, int n_heads, int n_req, int n_rows,
         const long long busy = n_req < n_rows ? n_req : n_rows;
         const long long some = ((long long)n_rows * G + p.nq - 1) / p.nq;
         units = (some > busy ? some : busy) * kv->n_kv_heads;
-        // A CTA costs about 11 us and 1.86 us per 128 tokens, one fits an SM; the join 3 us and its
+        // A CTA costs about 11 us and 1.86 us per 128 tokens (at head dim 128; smaller heads and tiles, whose
+        // tiles cost little less, are not told apart), one fits an SM; the join 3 us and its
         // records' way.  The S of the least time, as long as the longest CTA and as all of them on
         // 148 SMs: requests begin longest first and have ATTN_FILL of the tokens on average; a single one has
         // them all, and then CTAs come in whole rounds.  Measured (us, S = 1, 2, ...): 96 units of 8192

@@ -37,13 +37,14 @@
 // outputs go as whole rows, through V's slots before and after their use.
 //
 // Measured (heads of 128): 4096 rows behind 12288 tokens, 64 heads over 8,
-// 3.39 ms: 568 Tflop/s of attention, 1.14 Pflop/s of fp16 products, 0.68 of a
-// library's bf16 product.  8 prompts of up to 512 rows, 32 heads, 97 us; 32
-// requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 86 us.  Bound:
+// 3.43 ms: 561 Tflop/s of attention, 1.12 Pflop/s of fp16 products, 0.67 of a
+// library's bf16 product.  8 prompts of up to 512 rows, 32 heads, 96 us; 32
+// requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 84 us one call
+// after the other (89 us among other work).  Bound:
 // a tile takes 3700 cycles, of which 2048 are products.  The softmax warps'
 // chain is as long: waiting for and reading S 900, maxima 400, weights 1800 (64
 // of each thread's exponentials and conversions share a unit of 16 lanes), O
-// 450, and the next product starts behind it (one O fits TMEM).  A CTA costs
+// 450, and the next product starts behind it (one O fits TMEM at head dim 128).  A CTA costs
 // 11 us besides, mostly latencies one after the other: lookups, queries, first
 // tile, last product, output; hence short requests' distance from their floor.
 // Slower: one thread per query (-9 %); each half of the softmax warps on a tile
@@ -748,7 +749,8 @@ static cudaError_t launch_many(const Kv8AttnArgs &a, int tile_q, int tiles, cuda
         default: f = many_kernel<TYPE, 128>(tile_q); smem = MnSmem<128>::BYTES; break;
     }
     if ((long long)tiles * a.kv.n_kv_heads * a.S > INT_MAX) return cudaErrorInvalidValue;
-    // TMEM is allocated whole: one CTA per SM, so at least half of the shared memory is asked for
+    // TMEM is allocated whole, at smaller head dims too, where half of it would do: one CTA per SM, so at least
+    // half of the shared memory is asked for
     if (smem < 116 * 1024) smem = 116 * 1024;
     cudaError_t e = kv8_allow_smem((const void *)f, smem);
     if (e != cudaSuccess) return e;
