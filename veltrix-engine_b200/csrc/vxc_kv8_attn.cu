@@ -48,7 +48,7 @@ namespace cg = cooperative_groups;
 //
 // Measured (heads of 128): 33 requests of one row behind up to 16384 tokens, 64
 // heads over 8, 102 us one call after the other, 5.3 TB/s of the cache's bytes
-// (108 us among other work); 8 requests of 5 rows behind up to 768 tokens, 32
+// (108 to 113 us among other work); 8 requests of 5 rows behind up to 768 tokens, 32
 // heads, 13.9 us; 8 of one row, 32 heads of 64 over 4, 7.6 us.  Bound: bytes for
 // long contexts (issue slots 40 %, tensor pipe 33 % busy).  Short ones: a CTA's
 // latencies, about 4 us, and its warps' chain of scores, maxima, weights and

@@ -40,7 +40,7 @@
 // 3.43 ms: 561 Tflop/s of attention, 1.12 Pflop/s of fp16 products, 0.67 of a
 // library's bf16 product.  8 prompts of up to 512 rows, 32 heads, 96 us; 32
 // requests of 7 rows behind up to 4096 tokens, 64 heads over 8, 84 us one call
-// after the other (89 us among other work).  Bound:
+// after the other (89 to 91 us among other work).  Bound:
 // a tile takes 3700 cycles, of which 2048 are products.  The softmax warps'
 // chain is as long: waiting for and reading S 900, maxima 400, weights 1800 (64
 // of each thread's exponentials and conversions share a unit of 16 lanes), O
