@@ -83,9 +83,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // The splits of a request and head are joined by their cluster, through
 // distributed shared memory, while a cluster holds them all (a.S <= 8); else
 // they leave records in device memory for k_kv8_attn_join:
-// [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, l = sum of 2^(s - m), o = the split's own output.  (Every
-// partial output is divided by its own l and joined with weights 2^(m - M) l / L: sums of
-// 2^(s - m) v themselves would overflow for V within their number of tokens of the largest float.)
+// [row][head][S][4 + HD] = {m, l, -, -, o[HD]}, l = sum of 2^(s - m), o = the split's own output.  (A split's
+// output is divided by its own l and joined with weights 2^(m - M) l / L, a warp's by a power of two over l:
+// sums of 2^(s - m) v themselves would overflow for V within their number of tokens of the largest float.)
 template <int TYPE, int HD, int NQ>
 __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
     using P = Kv8Few<HD>;
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
         const float back = mv[i] == -INFINITY ? 0.0f : ex2(mv[i] - m[i] - KV8_HEAD);
-        const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];   // no token: 0; NaN stays
+        const float inv = kv8_pow2_under(l[i]);
         float *dst = so + (w * NQ + g + 8 * i) * (HD + 4);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -425,19 +425,23 @@ __global__ void __launch_bounds__(128, 2) k_kv8_attn_few(const Kv8AttnArgs a) {
         for (int k = 0; k < 4; k++) M = fmaxf(M, mw[k] = sml[(k * NQ + q) * 2]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            mw[k] = (mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M)) * sml[(k * NQ + q) * 2 + 1];
-            L += mw[k];
+            const float l = sml[(k * NQ + q) * 2 + 1];
+            mw[k] = mw[k] == -INFINITY ? 0.0f : ex2(mw[k] - M);
+            L += mw[k] * l;
+            mw[k] *= kv8_pow2_over(l);
         }
         const int row = rq.row0 + (q0 + q) / G, h = kvh * G + (q0 + q) % G;
         float *rec = cluster ? res + q * (HD + 4) : a.part + (((size_t)row * a.H + h) * a.S + split) * (HD + 4);
         float *out = a.out + (size_t)row * a.ldo + (size_t)h * HD;
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;   // no token: 0; NaN stays
 #pragma unroll
+        for (int k = 0; k < 4; k++) mw[k] *= inv;
+#pragma unroll
         for (int d = lane; d < HD; d += 32) {
             float x = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (mw[k] != 0.0f) x = fmaf(mw[k] * inv, so[(k * NQ + q) * (HD + 4) + d], x);
+                if (mw[k] != 0.0f) x = fmaf(mw[k], so[(k * NQ + q) * (HD + 4) + d], x);
             if (ns == 1) out[d] = x;
             else rec[4 + d] = x;
         }

@@ -111,6 +111,11 @@ __device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &h01, uint32_t &h2
     }
 }
 
+// A power of two 2^k over l >= 1 and at most twice as large, and its inverse; 0 gives 2^-126 and 2^126.  (l is at most
+// 2^36; NaN gives finite numbers.)
+__device__ __forceinline__ float kv8_pow2_over(float l) { return __uint_as_float((__float_as_uint(l) & 0x7F800000u) + 0x00800000u); }
+__device__ __forceinline__ float kv8_pow2_under(float l) { return __uint_as_float(0x7E800000u - (__float_as_uint(l) & 0x7F800000u)); }
+
 // A request's rows and tokens as the call's arguments and arrays allow them.
 struct Kv8Req {
     const int *table;
