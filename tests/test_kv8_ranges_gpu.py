@@ -145,3 +145,27 @@ def test_v_scales_apart_by_any_power(cuda, kind, new):
         e = rng.integers(-126, 118, nb)
         score = rng.integers(-120, 120, nb) if seed % 2 else np.full(nb, 100) - rng.integers(0, 4, nb) * 36
         run(cuda, kind, score, np.where(rng.random(nb) < 0.2, 0, 2.0 ** e), new=new, hd=128 if seed % 3 else 32, seed=seed)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,new,g,width", [(40, 1, 2, 0), (50, 6, 2, 0), (2000, 2, 4, 0), (30000, 1, 2, 0), (100, 30, 1, 0),
+                                                (100, 30, 2, 520), (300, 100, 2, 520), (2000, 40, 1, 520)])
+def test_nan_and_infinite_queries_stay_in_their_rows(cuda, kind, tokens, new, g, width):
+    """A query with a NaN or an infinity gives a row of NaN, whatever path it takes; all others are as without it."""
+    rng = np.random.default_rng(tokens)
+    hd, bs = 64, 16
+    nb = -(-tokens // bs)
+    d = Dev(cuda, kind, nb, bs, 1, hd, 1)
+    table = np.full((1, max(nb, width)), -1, np.int32)
+    table[0, :nb] = np.arange(nb)
+    q = rng.standard_normal((new, g, hd)).astype(np.float32)
+    row0, pos = np.array([0, new]), np.array([tokens - new])
+    want = d.attn(q, 0.1, table, row0, pos)
+    for bad in (np.nan, np.inf):
+        x = q.copy()
+        x[new // 2, g - 1, 5] = bad
+        got = d.attn(x, 0.1, table, row0, pos)
+        hit = np.zeros((new, g), bool)
+        hit[new // 2, g - 1] = True
+        assert np.all(np.isnan(got[hit]))
+        np.testing.assert_array_equal(got[~hit], want[~hit])
